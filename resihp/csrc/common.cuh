@@ -485,6 +485,29 @@ __device__ __forceinline__ bool wait_geq(const unsigned* p, unsigned target, int
   return true;
 }
 
+// ---- GEMM tiles and epilogues -----------------------------------------------------------
+
+// Output tile t of a tiles_m x tiles_n grid, eight tile rows at a time: the tiles that run
+// together share operand tiles in L2.
+__device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+  constexpr int kGroup = 8;
+  const int per_group = kGroup * tiles_n;
+  const int group = t / per_group;
+  const int first = group * kGroup;
+  const int size = min(tiles_m - first, kGroup);
+  const int in_group = t % per_group;
+  tm = first + in_group % size;
+  tn = in_group / size;
+}
+
+// Fire-and-forget C[0..3] += v in L2. Every element of C is added to by exactly one
+// thread of one CTA per launch, so the sum is the same single fp32 addition the
+// load-add-store epilogue performs (atomic f32 adds flush subnormals to zero).
+__device__ __forceinline__ void red_add_v4(float* p, float4 v) {
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+
 // ---- AdamW, one element (torch.optim.AdamW's formulation) -----------------------------
 // Shared by the stand-alone optimizer kernel and the fused DP-reduce + AdamW kernel, so
 // both paths round identically.

@@ -37,14 +37,6 @@ enum GemmEpilogue : int {
   kEpiRedF32 = 4,      // C(f32) += alpha * acc   (red.global.add: no load latency in the epilogue)
 };
 
-// Fire-and-forget C[0..3] += v in L2. Every element of C is added to by exactly one
-// thread of one CTA per launch, so the sum is the same single fp32 addition the
-// load-add-store epilogue performs (atomic f32 adds flush subnormals to zero).
-__device__ __forceinline__ void red_add_v4(float* p, float4 v) {
-  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-               : "memory");
-}
-
 struct GemmArgs {
   void* c;
   const void* r;
@@ -67,17 +59,6 @@ struct GemmShape {
   static constexpr int kSmem = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/;
   static constexpr int kTmemCols = 2 * BN;
 };
-
-__device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
-  constexpr int kGroup = 8;
-  const int per_group = kGroup * tiles_n;
-  const int group = t / per_group;
-  const int first = group * kGroup;
-  const int size = min(tiles_m - first, kGroup);
-  const int in_group = t % per_group;
-  tm = first + in_group % size;
-  tn = in_group / size;
-}
 
 // One thread's 32 consecutive accumulator columns (row ``row``, from column ``col0``)
 // through the epilogue into C.
@@ -496,6 +477,27 @@ CUtensorMap make_tma_2d_bf16(const void* base, int64_t rows, int64_t cols, int64
   cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+                           estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RESIHP_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", int(r));
+  return map;
+}
+
+// ``planes`` row-major [rows, cols] bf16 matrices ``plane_ld`` elements apart, tiled by
+// (box_cols, box_rows, 1): a box never reaches into the next plane, it reads zeros there.
+CUtensorMap make_tma_3d_bf16(const void* base, int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld,
+                             int box_cols, int box_rows) {
+  RESIHP_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0, "TMA base must be 16-byte aligned");
+  RESIHP_CHECK((ld * 2) % 16 == 0 && (plane_ld * 2) % 16 == 0, "TMA strides must be multiples of 16 bytes");
+  int dev = 0;
+  RESIHP_CUDA_CHECK(cudaGetDevice(&dev));
+  RESIHP_CUDA_CHECK(cudaSetDevice(dev));  // make the context current (see make_tma_2d_bf16)
+  CUtensorMap map;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * 2), static_cast<cuuint64_t>(plane_ld * 2)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
                            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RESIHP_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", int(r));

@@ -176,3 +176,47 @@ struct CopyDesc {
 void reshard_gather(const CopyDesc* descs_device, int ndesc, int64_t items, int* err, int num_sms, cudaStream_t st);
 
 }  // namespace resihp
+
+namespace resihp {
+
+// Dropout with a counter-based mask (dropout.cu). ``state``: device (seed, offset), or
+// nullptr for the two values given; ``drop``: of 65536 parts of the elements.
+void dropout(const void* x, const void* residual, void* out, bool bf16, int64_t n, int64_t first, uint64_t seed,
+             uint64_t offset, const int64_t* state, uint32_t drop, int num_sms, cudaStream_t st);
+
+// Sparse-MLP routing and row movements (moe.cu). counts: device scratch of
+// moe_blocks(tokens * k) x (experts + 1) ints.
+constexpr int kMoeMaxExperts = 1024;
+constexpr int kMoeMaxChoices = 16;
+int moe_blocks(int64_t pairs, int num_sms);
+void moe_route(const void* logits, bool bf16, int64_t ld, int tokens, int experts, int k, bool normalize,
+               float* weights, int* ids, int* counts, int* offsets, int* slots, int num_sms, cudaStream_t st);
+void moe_route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* ids,
+                   const float* dweights, void* dlogits, int tokens, int experts, int k, bool normalize,
+                   cudaStream_t st);
+void moe_plan(const int* ids, int64_t pairs, int start, int experts, int* counts, int* offsets, int* slots, int num_sms,
+              cudaStream_t st);
+// used: &offsets[experts]; places from there on belong to no expert.
+void moe_scatter(const void* x, const int* slots, const int* used, void* out, int tokens, int k, int d, int* err,
+                 cudaStream_t st);
+void moe_gather(const void* y, const float* weights, const void* residual, const int* slots, const int* used, void* out,
+                int tokens, int k, int d, int* err, cudaStream_t st);
+void moe_combine_bwd(const void* dout, const void* y, const float* weights, const int* slots, const int* used, void* dy,
+                     float* dweights, int tokens, int k, int d, int* err, cudaStream_t st);
+
+// Products grouped by expert (grouped.cu): group g owns the rows offsets[g]..offsets[g + 1].
+struct GroupedShape {
+  const int* offsets;  // device, [groups + 1]
+  int groups, rows;    // rows: of the row operands; those behind the last group's give zeros
+  int n, k;            // output columns, reduction length (wgrad: output rows x columns)
+};
+// c[r, n] = sum_k a[r, k] w[g(r), n, k] (w_mn: w[g(r), k, n]), bf16.
+void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t w_group, bool w_mn, void* c,
+                  int64_t ldc, const GroupedShape& s, int* err, cudaStream_t st);
+// c[g, n, k] (+)= sum over the group's rows of dy[r, n] x[r, k], fp32 [groups, n, k] contiguous.
+void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, float* c, bool accumulate,
+                   const GroupedShape& s, int* err, cudaStream_t st);
+CUtensorMap make_tma_3d_bf16(const void* base, int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld,
+                             int box_cols, int box_rows);
+
+}  // namespace resihp

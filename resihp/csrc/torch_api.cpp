@@ -278,6 +278,189 @@ torch::Tensor attn_bwd_t(torch::Tensor qkv, torch::Tensor out, torch::Tensor dou
 }
 
 
+// ---- dropout --------------------------------------------------------------------------
+
+torch::Tensor dropout_t(torch::Tensor x, c10::optional<torch::Tensor> residual, int64_t drop, int64_t seed,
+                        int64_t offset, c10::optional<torch::Tensor> state, int64_t first) {
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous(), "dropout: x must be a contiguous CUDA tensor");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat, "dropout: x must be bf16 or fp32");
+  const void* rp = nullptr;
+  if (residual.has_value()) {
+    TORCH_CHECK(residual->device() == x.device() && residual->scalar_type() == x.scalar_type() &&
+                    residual->sizes() == x.sizes() && residual->is_contiguous(),
+                "dropout: residual must match x");
+    rp = residual->data_ptr();
+  }
+  const int64_t* sp = nullptr;
+  if (state.has_value()) {
+    TORCH_CHECK(state->device() == x.device() && state->scalar_type() == at::kLong && state->numel() == 2 &&
+                    state->is_contiguous(), "dropout: the seed tensor must be int64 [2] beside x");
+    sp = state->data_ptr<int64_t>();
+  }
+  TORCH_CHECK(drop >= 0 && drop <= 65536, "dropout threshold out of range");
+  c10::cuda::CUDAGuard guard(x.device());
+  auto out = torch::empty_like(x);
+  dropout(x.data_ptr(), rp, out.data_ptr(), x.scalar_type() == at::kBFloat16, x.numel(), first, uint64_t(seed),
+          uint64_t(offset), sp, uint32_t(drop), sms(x), cur_stream());
+  return out;
+}
+
+// ---- sparse MLP: routing and row movements ----------------------------------------------
+
+static void check_int32(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous(), name,
+              " must be a contiguous int32 tensor on the rows' device");
+}
+
+static void check_rows_count(int64_t rows, int64_t k) {
+  TORCH_CHECK(rows * k <= INT32_MAX, "tokens * k passes 31 bits");
+}
+
+std::vector<torch::Tensor> moe_route_t(torch::Tensor logits, int64_t k, bool normalize) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, "logits must be CUDA [tokens, experts]");
+  TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat, "logits must be bf16 or fp32");
+  const int64_t t = logits.size(0), e = logits.size(1);
+  check_rows_count(t, k);
+  c10::cuda::CUDAGuard guard(logits.device());
+  const auto ints = logits.options().dtype(torch::kInt);
+  auto weights = torch::empty({t, k}, logits.options().dtype(torch::kFloat));
+  auto ids = torch::empty({t, k}, ints);
+  auto slots = torch::empty({t, k}, ints);
+  auto offsets = torch::empty({e + 1}, ints);
+  auto counts = torch::empty({moe_blocks(t * k, sms(logits)), e + 1}, ints);
+  moe_route(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0), int(t), int(e), int(k), normalize,
+            weights.data_ptr<float>(), ids.data_ptr<int>(), counts.data_ptr<int>(), offsets.data_ptr<int>(),
+            slots.data_ptr<int>(), sms(logits), cur_stream());
+  return {weights, ids, offsets, slots};
+}
+
+torch::Tensor moe_route_bwd_t(torch::Tensor logits, torch::Tensor weights, torch::Tensor ids, torch::Tensor dweights,
+                              bool normalize) {
+  const int64_t t = logits.size(0), e = logits.size(1), k = ids.size(1);
+  TORCH_CHECK(dweights.device() == logits.device() && dweights.scalar_type() == at::kFloat && dweights.is_contiguous() &&
+                  dweights.numel() == t * k, "weight gradients must be contiguous fp32 [tokens, k]");
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto out = torch::empty({t, e}, logits.options());
+  moe_route_bwd(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0), weights.data_ptr<float>(),
+                ids.data_ptr<int>(), dweights.data_ptr<float>(), out.data_ptr(), int(t), int(e), int(k), normalize,
+                cur_stream());
+  return out;
+}
+
+std::vector<torch::Tensor> moe_plan_t(torch::Tensor ids, int64_t experts, int64_t start) {
+  TORCH_CHECK(ids.is_cuda() && ids.scalar_type() == at::kInt && ids.is_contiguous(), "ids must be contiguous int32 CUDA");
+  TORCH_CHECK(start >= INT32_MIN && start <= INT32_MAX, "first expert out of range");
+  TORCH_CHECK(experts >= 1 && experts <= kMoeMaxExperts, "expert count out of range");
+  check_rows_count(ids.numel(), 1);
+  c10::cuda::CUDAGuard guard(ids.device());
+  auto offsets = torch::empty({experts + 1}, ids.options());
+  auto slots = torch::empty_like(ids);
+  auto counts = torch::empty({moe_blocks(ids.numel(), sms(ids)), experts + 1}, ids.options());
+  moe_plan(ids.data_ptr<int>(), ids.numel(), int(start), int(experts), counts.data_ptr<int>(), offsets.data_ptr<int>(),
+           slots.data_ptr<int>(), sms(ids), cur_stream());
+  return {offsets, slots};
+}
+
+static void check_plan(const torch::Tensor& rows, const torch::Tensor& offsets, const torch::Tensor& slots) {
+  check_int32(offsets, rows, "offsets");
+  check_int32(slots, rows, "slots");
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() >= 2 && slots.dim() == 2 && slots.size(1) >= 1,
+              "a plan is offsets [experts + 1] and slots [tokens, k]");
+  check_rows_count(slots.size(0), slots.size(1));
+}
+
+torch::Tensor moe_scatter_t(torch::Tensor x, torch::Tensor offsets, torch::Tensor slots) {
+  check_plan(x, offsets, slots);
+  check_rows(x, x.size(-1), "x");
+  TORCH_CHECK(x.size(0) == slots.size(0), "x must have a row per token");
+  c10::cuda::CUDAGuard guard(x.device());
+  auto out = torch::empty({slots.numel(), x.size(1)}, x.options());
+  moe_scatter(x.data_ptr(), slots.data_ptr<int>(), offsets.data_ptr<int>() + offsets.numel() - 1, out.data_ptr(),
+              int(x.size(0)), int(slots.size(1)), int(x.size(1)), error_word(x.device()), cur_stream());
+  return out;
+}
+
+static const float* check_weights(const c10::optional<torch::Tensor>& w, const torch::Tensor& slots) {
+  if (!w.has_value()) return nullptr;
+  TORCH_CHECK(w->device() == slots.device() && w->scalar_type() == at::kFloat && w->is_contiguous() &&
+                  w->sizes() == slots.sizes(), "weights must be contiguous fp32 [tokens, k]");
+  return w->data_ptr<float>();
+}
+
+torch::Tensor moe_gather_t(torch::Tensor y, c10::optional<torch::Tensor> weights, torch::Tensor offsets,
+                           torch::Tensor slots, c10::optional<torch::Tensor> residual) {
+  check_plan(y, offsets, slots);
+  check_rows(y, y.size(-1), "y");
+  TORCH_CHECK(y.size(0) == slots.numel(), "y must have a row per (token, choice) pair");
+  const float* wp = check_weights(weights, slots);
+  const void* rp = nullptr;
+  if (residual.has_value()) {
+    check_rows(*residual, y.size(1), "residual");
+    TORCH_CHECK(residual->size(0) == slots.size(0) && residual->device() == y.device(), "residual must have a row per token");
+    rp = residual->data_ptr();
+  }
+  c10::cuda::CUDAGuard guard(y.device());
+  auto out = torch::empty({slots.size(0), y.size(1)}, y.options());
+  moe_gather(y.data_ptr(), wp, rp, slots.data_ptr<int>(), offsets.data_ptr<int>() + offsets.numel() - 1, out.data_ptr(),
+             int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), cur_stream());
+  return out;
+}
+
+std::vector<torch::Tensor> moe_combine_bwd_t(torch::Tensor dout, torch::Tensor y, c10::optional<torch::Tensor> weights,
+                                             torch::Tensor offsets, torch::Tensor slots) {
+  check_plan(dout, offsets, slots);
+  check_rows(dout, y.size(-1), "dout");
+  check_rows(y, y.size(-1), "y");
+  TORCH_CHECK(dout.size(0) == slots.size(0) && y.size(0) == slots.numel() && y.device() == dout.device(), "combine shapes");
+  const float* wp = check_weights(weights, slots);
+  c10::cuda::CUDAGuard guard(dout.device());
+  auto dy = torch::empty_like(y);
+  auto dw = torch::empty(slots.sizes(), y.options().dtype(torch::kFloat));
+  moe_combine_bwd(dout.data_ptr(), y.data_ptr(), wp, slots.data_ptr<int>(),
+                  offsets.data_ptr<int>() + offsets.numel() - 1, dy.data_ptr(), dw.data_ptr<float>(),
+                  int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), cur_stream());
+  return {dy, dw};
+}
+
+// ---- products grouped by expert -----------------------------------------------------------
+
+static GroupedShape grouped_shape(const torch::Tensor& rows, const torch::Tensor& offsets, int64_t n, int64_t k) {
+  check_int32(offsets, rows, "offsets");
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() >= 2, "offsets must be [groups + 1]");
+  TORCH_CHECK(rows.size(0) <= INT32_MAX - 512 && n <= INT32_MAX - 512 && k <= INT32_MAX - 512, "grouped product too large");
+  return GroupedShape{offsets.data_ptr<int>(), int(offsets.numel() - 1), int(rows.size(0)), int(n), int(k)};
+}
+
+// a [rows, K] times w [groups, N, K] transposed, or with w_mn times w [groups, K, N].
+torch::Tensor grouped_rows_t(torch::Tensor a, torch::Tensor w, bool w_mn, torch::Tensor offsets) {
+  check_cuda_bf16(a, "rows");
+  check_cuda_bf16(w, "weights");
+  TORCH_CHECK(a.dim() == 2 && w.dim() == 3 && a.stride(1) == 1 && w.stride(2) == 1 && a.device() == w.device(),
+              "grouped product needs [rows, K] and [groups, N, K] with unit inner strides on one device");
+  const int64_t k = w_mn ? w.size(1) : w.size(2), n = w_mn ? w.size(2) : w.size(1);
+  TORCH_CHECK(a.size(1) == k && w.size(0) == offsets.numel() - 1, "grouped product: sizes differ");
+  const GroupedShape s = grouped_shape(a, offsets, n, k);
+  c10::cuda::CUDAGuard guard(a.device());
+  auto c = torch::empty({a.size(0), n}, a.options());
+  grouped_rows(a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(1), w.stride(0), w_mn, c.data_ptr(), n, s,
+               error_word(a.device()), cur_stream());
+  return c;
+}
+
+void grouped_wgrad_t(torch::Tensor dy, torch::Tensor x, torch::Tensor offsets, torch::Tensor out, bool accumulate) {
+  check_cuda_bf16(dy, "dy");
+  check_cuda_bf16(x, "x");
+  TORCH_CHECK(dy.dim() == 2 && x.dim() == 2 && dy.stride(1) == 1 && x.stride(1) == 1 && dy.size(0) == x.size(0) &&
+                  dy.device() == x.device(), "grouped wgrad needs dy [rows, N] and x [rows, K]");
+  const GroupedShape s = grouped_shape(dy, offsets, dy.size(1), x.size(1));
+  TORCH_CHECK(out.device() == dy.device() && out.scalar_type() == at::kFloat && out.is_contiguous() && out.dim() == 3 &&
+                  out.size(0) == s.groups && out.size(1) == s.n && out.size(2) == s.k,
+              "grouped weight gradient must be contiguous fp32 [groups, N, K]");
+  c10::cuda::CUDAGuard guard(dy.device());
+  grouped_wgrad(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), out.data_ptr<float>(), accumulate, s,
+                error_word(dy.device()), cur_stream());
+}
+
 // ---- debugging aid: native backtrace on SIGSEGV ---------------------------------------
 
 static void crash_handler(int sig) {
@@ -508,6 +691,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("xent_grad", &resihp::xent_grad_t);
   m.def("attn_fwd", &resihp::attn_fwd_t);
   m.def("attn_bwd", &resihp::attn_bwd_t);
+  m.def("dropout", &resihp::dropout_t);
+  m.def("moe_route", &resihp::moe_route_t);
+  m.def("moe_route_bwd", &resihp::moe_route_bwd_t);
+  m.def("moe_plan", &resihp::moe_plan_t);
+  m.def("moe_scatter", &resihp::moe_scatter_t);
+  m.def("moe_gather", &resihp::moe_gather_t);
+  m.def("moe_combine_bwd", &resihp::moe_combine_bwd_t);
+  m.def("grouped_rows", &resihp::grouped_rows_t);
+  m.def("grouped_wgrad", &resihp::grouped_wgrad_t);
   m.def("install_crash_handler", &resihp::install_crash_handler);
   m.def("symm_alloc", &resihp::symm_alloc_t);
   m.def("symm_open", &resihp::symm_open_t);

@@ -6,3 +6,4 @@ CPU tensors; there is no other path.
 
 from . import _ext  # noqa: F401
 from .gemm import KernelError, check_device_errors, linear, linear_dgrad, linear_wgrad  # noqa: F401
+from .gemm import grouped_dgrad, grouped_linear, grouped_wgrad  # noqa: F401

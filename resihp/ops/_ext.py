@@ -43,6 +43,8 @@ def _load():
 KERNELS_PER_CALL = {
     "gemm": 1, "rmsnorm_fwd": 1, "rmsnorm_bwd": 2, "rope": 1, "swiglu_fwd": 1, "swiglu_bwd": 1,
     "adamw": 1, "embedding_fwd": 1, "embedding_bwd": 2, "xent_stats": 1, "xent_grad": 1,
+    "dropout": 1, "moe_route": 2, "moe_route_bwd": 1, "moe_plan": 2, "moe_scatter": 1, "moe_gather": 1,
+    "moe_combine_bwd": 1, "grouped_rows": 1, "grouped_wgrad": 1,
     "attn_fwd": 1, "attn_bwd": 3, "ag_gemm": 1, "gemm_rs": 1, "dp_allreduce_adamw": 1, "reshard_gather": 1,
 }
 

@@ -26,7 +26,9 @@ from torch.nn import functional as F
 
 from . import _ext
 from .gemm import linear as _gemm_linear
-from .gemm import linear_dgrad, linear_wgrad
+from .gemm import grouped_dgrad, grouped_wgrad, linear_dgrad, linear_wgrad  # noqa: F401
+from .dropout import dropout  # noqa: F401
+from .moe import MoePlan, grouped_linear, moe_combine, moe_dispatch, moe_plan, moe_route  # noqa: F401
 
 
 def _k():
@@ -217,6 +219,27 @@ def swiglu(gu):
         return _SwiGLU.apply(gu)
     g, u = gu.chunk(2, dim=-1)
     return F.silu(g) * u
+
+
+# ---------------------------------------------------------------------------------------
+# sparse MLP (mixture of experts)
+# ---------------------------------------------------------------------------------------
+
+
+def moe_swiglu(x, w_router, w_gate_up, w_down, k, *, normalize=True, residual=None, grads=None):
+    """A sparse SwiGLU MLP over ``x [T, d]``: every token's ``k`` experts, weighted, plus ``residual``.
+
+    ``w_router [E, d]`` gives the router logits (FP32 sums of ``x``'s products, rounded to its
+    dtype), ``w_gate_up [E, 2F, d]`` and ``w_down [E, d, F]`` are the experts' fused gate / up
+    and down projections. ``grads``: the FP32 main-grad buffers of the three weights in that
+    order (CUDA bf16; see :func:`linear`). On the kernels the router takes a multiple of 8
+    experts (its logits are a GEMM's output). The steps are :mod:`resihp.ops.moe`'s.
+    """
+    g_router, g_gate_up, g_down = grads if grads is not None else (None, None, None)
+    weights, _, plan = moe_route(linear(x, w_router, g_router), k, normalize)
+    gu = grouped_linear(moe_dispatch(x, plan), w_gate_up, plan.offsets, g_gate_up)
+    y = grouped_linear(swiglu(gu), w_down, plan.offsets, g_down)
+    return moe_combine(y, weights, plan, residual)
 
 
 # ---------------------------------------------------------------------------------------

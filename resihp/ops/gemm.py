@@ -87,6 +87,107 @@ def linear_wgrad(dy: torch.Tensor, x: torch.Tensor, out: torch.Tensor | None = N
     return out
 
 
+# ---------------------------------------------------------------------------------------
+# products grouped by expert (``csrc/grouped.cu``)
+# ---------------------------------------------------------------------------------------
+
+MAX_GROUPS = 1024
+
+
+def check_groups(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> None:
+    """Refuse operands of a grouped product ``x [R, K]``, ``w [E, N, K]``, ``offsets [E + 1]``."""
+    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2]:
+        raise ValueError(f"a grouped product takes rows [R, K] and weights [E, N, K], got {list(x.shape)} and {list(w.shape)}")
+    if x.dtype != w.dtype or x.device != w.device:
+        raise ValueError(f"rows ({x.dtype}, {x.device}) and weights ({w.dtype}, {w.device}) must match")
+    _check_offsets(x, offsets, w.shape[0])
+    _check_widths(x, w.shape[1], w.shape[2])
+
+
+def _check_offsets(x: torch.Tensor, offsets: torch.Tensor, groups: int) -> None:
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.device != x.device:
+        raise ValueError("offsets must be an int32 vector on the rows' device")
+    if offsets.numel() != groups + 1 or not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"{groups} groups need {groups + 1} offsets (1 to {MAX_GROUPS} groups), got {offsets.numel()}")
+
+
+def _check_widths(x: torch.Tensor, n: int, k: int) -> None:
+    if n < 1 or k < 1:
+        raise ValueError("a grouped product needs widths of at least 1")
+    if _cuda(x) and (n % 8 or k % 8):
+        raise ValueError(f"the bf16 kernels need widths that are multiples of 8, got {n} and {k}")
+    if x.is_cuda and x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"grouped products run in bf16 or fp32, not {x.dtype}")
+
+
+def _tiles(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as TMA reads it: unit inner stride, 16-byte aligned base and outer strides (which
+    no two rows may share); anything else is copied."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+def _bounds(offsets: torch.Tensor, rows: int) -> list[int]:
+    """The groups' first rows on the host, clamped like the kernels do (FP32 path)."""
+    out, last = [0], 0
+    for v in offsets.tolist()[1:]:
+        last = max(last, min(max(v, 0), rows))
+        out.append(last)
+    return out
+
+
+def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """``y[r] = w[g(r)] @ x[r]``: rows ``offsets[g] .. offsets[g + 1]`` of ``x [R, K]`` times the
+    group's ``w[g] [N, K]``; rows behind the last group give zeros. ``offsets`` (int32, first
+    entry 0, not decreasing) stays on the device: lengths, empty groups among them, are read
+    by the kernel. Entries that decrease or pass ``R`` are clamped and reported by
+    :func:`check_device_errors`."""
+    check_groups(x, w, offsets)
+    if _cuda(x):
+        return _ext.require().grouped_rows(_tiles(x), _tiles(w), False, offsets.contiguous())
+    at = _bounds(offsets, x.shape[0])
+    parts = [torch.nn.functional.linear(x[a:b], w[g]) for g, (a, b) in enumerate(zip(at, at[1:]))]
+    return torch.cat(parts + [x.new_zeros(x.shape[0] - at[-1], w.shape[1])])
+
+
+def grouped_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """``dx[r] = w[g(r)]^T @ dy[r]``: the input gradient of :func:`grouped_linear`."""
+    check_groups(dy, w.transpose(1, 2) if w.dim() == 3 else w, offsets)
+    if _cuda(dy):
+        return _ext.require().grouped_rows(_tiles(dy), _tiles(w), True, offsets.contiguous())
+    at = _bounds(offsets, dy.shape[0])
+    parts = [dy[a:b] @ w[g] for g, (a, b) in enumerate(zip(at, at[1:]))]
+    return torch.cat(parts + [dy.new_zeros(dy.shape[0] - at[-1], w.shape[2])])
+
+
+def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor | None = None,
+                  accumulate: bool = False) -> torch.Tensor:
+    """``dw[g] = sum over the group's rows of dy[r] x[r]^T`` in FP32 ``[E, N, K]``: the weight
+    gradient of :func:`grouped_linear`, added into ``out`` with ``accumulate``."""
+    groups = offsets.numel() - 1
+    if dy.dim() != 2 or x.dim() != 2 or dy.shape[0] != x.shape[0] or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError("a grouped weight gradient takes dy [R, N] and x [R, K] of one dtype and device")
+    _check_offsets(dy, offsets, groups)
+    _check_widths(dy, dy.shape[1], x.shape[1])
+    shape = (groups, dy.shape[1], x.shape[1])
+    if out is None:
+        out, accumulate = torch.empty(shape, dtype=torch.float32, device=dy.device), False
+    elif out.shape != shape or out.dtype != torch.float32 or out.device != dy.device or not out.is_contiguous():
+        raise ValueError(f"the weight gradient goes into a contiguous fp32 {list(shape)} on the rows' device")
+    if _cuda(dy):
+        _ext.require().grouped_wgrad(_tiles(dy), _tiles(x), offsets.contiguous(), out, accumulate)
+        return out
+    at = _bounds(offsets, dy.shape[0])
+    for g, (a, b) in enumerate(zip(at, at[1:])):
+        product = dy[a:b].t().float() @ x[a:b].float()
+        if accumulate:
+            out[g].add_(product)
+        else:
+            out[g].copy_(product)
+    return out
+
+
 #: Codes a kernel records in its device's error word (``ErrorCode`` in csrc/common.cuh).
 ERROR_CODES = {
     1: "TMA producer waited past its budget for a free shared-memory stage",

@@ -1,0 +1,256 @@
+"""Sparse (mixture-of-experts) MLP: routing, row movements and per-expert linear layers.
+
+The steps of one block, in order, over ``T`` tokens, ``E`` experts and ``k`` choices per token::
+
+    weights, ids, plan = moe_route(logits, k)                 # logits [T, E]
+    rows = moe_dispatch(x, plan)                              # [T * k, d], sorted by expert
+    gu = grouped_linear(rows, w_gate_up, plan.offsets, g)     # one linear layer per expert
+    y = grouped_linear(swiglu(gu), w_down, plan.offsets, g)
+    out = moe_combine(y, weights, plan, residual=x)           # [T, d]
+
+:func:`moe_swiglu` is that block in one call. Nothing waits for the host: the experts' row
+counts stay on the device, and every kernel reads them there. A choice that no expert takes
+(``-inf`` logits, ids outside ``start .. start + experts``) moves no weight: its place lies
+behind the last expert's rows, which are zero, and :func:`moe_combine` leaves it out.
+
+As elsewhere in this package bf16 CUDA tensors run the kernels (``csrc/moe.cu``,
+``csrc/grouped.cu``) and FP32 rows the plain torch expressions; the router's logits run its
+kernel on every CUDA device in bf16 or FP32. (No counterpart in the reference, whose blocks
+are dense.)
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _ext
+from .gemm import MAX_GROUPS, _cuda, check_groups, grouped_dgrad, grouped_wgrad
+from .gemm import grouped_linear as _grouped_linear
+
+MAX_CHOICES = 16
+
+
+class MoePlan(NamedTuple):
+    """Where the ``T * k`` (token, choice) pairs go when sorted by expert, token, choice.
+
+    ``offsets`` (int32 ``[E + 1]``): expert ``e`` owns the rows ``offsets[e] .. offsets[e + 1]``.
+    ``slots`` (int32 ``[T, k]``): each pair's row; pairs of no expert have the rows from
+    ``offsets[E]`` on. Every row belongs to exactly one pair.
+    """
+
+    offsets: torch.Tensor
+    slots: torch.Tensor
+
+
+# ---------------------------------------------------------------------------------------
+# routing
+# ---------------------------------------------------------------------------------------
+
+
+def _plan_torch(ids, experts: int, start: int) -> MoePlan:
+    local = ids.reshape(-1).long() - start
+    key = torch.where((local < 0) | (local >= experts), experts, local)
+    order = key.argsort(stable=True)
+    slots = torch.empty_like(order)
+    slots[order] = torch.arange(order.numel(), device=ids.device)
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device=ids.device)
+    offsets[1:] = torch.bincount(key, minlength=experts + 1)[:experts].cumsum(0)
+    return MoePlan(offsets, slots.to(torch.int32).view(ids.shape))
+
+
+def _route_torch(logits, k: int, normalize: bool):
+    x = logits.float()
+    top, ids = x.sort(dim=1, descending=True, stable=True)
+    top, ids = top[:, :k], ids[:, :k]
+    allowed = top != float("-inf")
+    among = top if normalize else x
+    m = among.amax(1, keepdim=True).detach()
+    m = torch.where(m == float("-inf"), torch.zeros_like(m), m)
+    total = (among - m).exp().sum(1, keepdim=True)
+    weights = torch.where(allowed, (top - m).exp(), torch.zeros_like(top)) / total.masked_fill(total == 0, 1.0)
+    return weights, torch.where(allowed, ids, torch.full_like(ids, -1)).to(torch.int32)
+
+
+class _Route(Function):
+    @staticmethod
+    def forward(ctx, logits, k, normalize):
+        weights, ids, offsets, slots = _ext.require().moe_route(logits, k, normalize)
+        ctx.save_for_backward(logits, weights, ids)
+        ctx.normalize = normalize
+        ctx.mark_non_differentiable(ids, offsets, slots)
+        return weights, ids, offsets, slots
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, *_):
+        logits, weights, ids = ctx.saved_tensors
+        return _ext.require().moe_route_bwd(logits, weights, ids, dweights.contiguous(), ctx.normalize), None, None
+
+
+def moe_route(logits, k: int, normalize: bool = True):
+    """The ``k`` experts of every token: ``(weights, ids, plan)`` from router logits ``[T, E]``.
+
+    Choice ``j`` is the token's ``j``-th largest logit, the lowest expert first among equal
+    ones. ``weights`` (FP32 ``[T, k]``) are the softmax over the chosen experts (``normalize``)
+    or the chosen experts' part of the softmax over all; gradients flow through them. A logit
+    of ``-inf`` is an expert the token may not use: it is never chosen, and where fewer than
+    ``k`` are left the remaining choices are ``-1`` with weight 0 -- a token without any
+    allowed expert (padding) takes no row. ``ids`` is int32 ``[T, k]``, ``plan`` sorts the
+    choices (:class:`MoePlan`). NaN sorts above everything, and its token's weights are NaN.
+    """
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"router logits must be bf16 or fp32 [T, E], got {logits.dtype} {list(logits.shape)}")
+    experts = logits.shape[1]
+    if not 1 <= experts <= MAX_GROUPS or not 1 <= k <= min(experts, MAX_CHOICES):
+        raise ValueError(f"{k} choices of {experts} experts: 1 to {MAX_CHOICES} choices, no more than experts, "
+                         f"of 1 to {MAX_GROUPS} experts")
+    if logits.is_cuda:
+        rows = logits if logits.stride(1) == 1 else logits.contiguous()
+        weights, ids, offsets, slots = _Route.apply(rows, int(k), bool(normalize))
+        return weights, ids, MoePlan(offsets, slots)
+    weights, ids = _route_torch(logits, k, normalize)
+    return weights, ids, _plan_torch(ids, experts, 0)
+
+
+def moe_plan(ids, experts: int, start: int = 0) -> MoePlan:
+    """The plan of choices made elsewhere: ``ids`` int32 ``[T, k]``, the experts ``start ..
+    start + experts`` (this rank's); any other id is a choice that no expert here takes."""
+    if ids.dim() != 2 or ids.dtype != torch.int32 or ids.shape[1] < 1:
+        raise ValueError(f"expert ids must be int32 [T, k], got {ids.dtype} {list(ids.shape)}")
+    if not 1 <= experts <= MAX_GROUPS or not -(2**31) <= start < 2**31:
+        raise ValueError(f"a plan takes 1 to {MAX_GROUPS} experts from a 32-bit start, got {experts} from {start}")
+    if ids.is_cuda:
+        return MoePlan(*_ext.require().moe_plan(ids.contiguous(), int(experts), int(start)))
+    return _plan_torch(ids, experts, start)
+
+
+# ---------------------------------------------------------------------------------------
+# row movements
+# ---------------------------------------------------------------------------------------
+
+
+def _check_plan(rows, plan: MoePlan) -> tuple[torch.Tensor, torch.Tensor]:
+    offsets, slots = plan
+    if slots.dim() != 2 or slots.shape[1] < 1 or offsets.dim() != 1 or offsets.numel() < 2:
+        raise ValueError("a plan is offsets [E + 1] and slots [T, k]")
+    if slots.dtype != torch.int32 or offsets.dtype != torch.int32:
+        raise ValueError("a plan's offsets and slots must be int32")
+    if slots.device != rows.device or offsets.device != rows.device:
+        raise ValueError("a plan must lie on its rows' device")
+    if rows.dim() != 2 or rows.shape[1] < 1:
+        raise ValueError(f"rows must be [rows, d] with d of at least 1, got {list(rows.shape)}")
+    if rows.is_cuda and rows.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"rows move in bf16 or fp32, not {rows.dtype}")
+    return offsets.contiguous(), slots.contiguous()
+
+
+class _Dispatch(Function):
+    @staticmethod
+    def forward(ctx, x, offsets, slots):
+        ctx.save_for_backward(offsets, slots)
+        return _ext.require().moe_scatter(x, offsets, slots)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        offsets, slots = ctx.saved_tensors
+        return _ext.require().moe_gather(dy.contiguous(), None, offsets, slots, None), None, None
+
+
+def moe_dispatch(x, plan: MoePlan):
+    """Token rows ``x [T, d]`` in the plan's order ``[T * k, d]``: ``y[slots[t, j]] = x[t]``, zeros
+    in the rows of choices that no expert takes."""
+    offsets, slots = _check_plan(x, plan)
+    if x.shape[0] != slots.shape[0]:
+        raise ValueError(f"{x.shape[0]} rows for a plan of {slots.shape[0]} tokens")
+    if _cuda(x):
+        return _Dispatch.apply(x.contiguous(), offsets, slots)
+    at = slots.long()
+    rows = x[:, None, :] * (at < offsets[-1])[..., None].to(x.dtype)
+    return torch.zeros_like(rows).view(-1, x.shape[1]).index_copy(0, at.reshape(-1), rows.reshape(-1, x.shape[1]))
+
+
+class _Combine(Function):
+    @staticmethod
+    def forward(ctx, y, weights, offsets, slots, residual):
+        ctx.save_for_backward(y, weights, offsets, slots)
+        ctx.has_residual = residual is not None
+        return _ext.require().moe_gather(y, weights, offsets, slots, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        y, weights, offsets, slots = ctx.saved_tensors
+        dout = dout.contiguous()
+        dy = dw = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            dy, dw = _ext.require().moe_combine_bwd(dout, y, weights, offsets, slots)
+        return dy, dw, None, None, (dout if ctx.has_residual else None)
+
+
+def moe_combine(y, weights, plan: MoePlan, residual=None):
+    """``out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]]`` over the choices that an
+    expert takes, in FP32 and rounded once; ``y [T * k, d]``, ``weights`` FP32 ``[T, k]``."""
+    offsets, slots = _check_plan(y, plan)
+    if y.shape[0] != slots.numel():
+        raise ValueError(f"{y.shape[0]} rows for a plan of {slots.numel()} choices")
+    if weights.shape != slots.shape or weights.dtype != torch.float32 or weights.device != y.device:
+        raise ValueError(f"weights must be fp32 {list(slots.shape)} beside the rows")
+    if residual is not None and (residual.shape != (slots.shape[0], y.shape[1]) or residual.dtype != y.dtype
+                                 or residual.device != y.device):
+        raise ValueError("the residual must be [T, d] in the rows' dtype, beside them")
+    if _cuda(y):
+        return _Combine.apply(y.contiguous(), weights.contiguous(), offsets, slots,
+                              None if residual is None else residual.contiguous())
+    at = slots.long()
+    kept = (at < offsets[-1])[..., None]
+    rows = torch.where(kept, y[at.reshape(-1)].view(*at.shape, -1), torch.zeros((), dtype=y.dtype, device=y.device))
+    out = (rows * weights[..., None]).sum(1)
+    return out if residual is None else residual + out
+
+
+# ---------------------------------------------------------------------------------------
+# per-expert linear layers
+# ---------------------------------------------------------------------------------------
+
+
+class _GroupedLinear(Function):
+    @staticmethod
+    def forward(ctx, x, w, offsets, main_grad):
+        ctx.save_for_backward(x, w, offsets)
+        ctx.main_grad = main_grad
+        return _grouped_linear(x, w, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, offsets = ctx.saved_tensors
+        dy = dy.contiguous()
+        dx = grouped_dgrad(dy, w, offsets) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.main_grad is not None:
+            grouped_wgrad(dy, x, offsets, out=ctx.main_grad, accumulate=True)
+        elif ctx.needs_input_grad[1]:
+            dw = grouped_wgrad(dy, x, offsets).to(w.dtype)
+        return dx, dw, None, None
+
+
+def grouped_linear(x, w, offsets, main_grad=None):
+    """One linear layer per expert: ``y[r] = w[e(r)] @ x[r]`` for the rows ``offsets[e] ..
+    offsets[e + 1]`` of ``x [R, K]``, ``w [E, N, K]``; zeros behind the last expert's rows.
+
+    CUDA bf16: tcgen05 products, widths multiples of 8; the weight gradient is accumulated
+    into ``main_grad`` (FP32 ``[E, N, K]``) where one is given, as :func:`linear` does, and
+    is ``w``'s gradient otherwise. Rows behind the last expert get a zero gradient.
+    """
+    check_groups(x, w, offsets)
+    if main_grad is not None and (main_grad.shape != w.shape or main_grad.dtype != torch.float32
+                                  or main_grad.device != w.device or not main_grad.is_contiguous()):
+        raise ValueError(f"main_grad must be a contiguous fp32 {list(w.shape)} beside the weights")
+    if not _cuda(x):
+        return _grouped_linear(x, w, offsets)
+    return _GroupedLinear.apply(x, w, offsets, main_grad)
