@@ -331,6 +331,29 @@ __device__ __forceinline__ void l2_prefetch_bulk(const void* src, uint32_t bytes
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 
+// A tile of fp32 from this CTA's shared memory to its place in a 3-D tensor map (stored, or
+// added element by element), in the thread's current bulk group. What lies past the map's
+// edges is left out; ``x`` is a multiple of 4 elements (16 bytes) and nothing is negative.
+__device__ __forceinline__ void tma_store_3d_f32(const CUtensorMap* map, const void* src, int x, int y, int z,
+                                                 int* err = nullptr) {
+  if (!bounds_ok((x & 3) == 0 && x >= 0 && y >= 0 && z >= 0 && (smem_u32(src) & 127u) == 0, err)) return;
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void tma_add_3d_f32(const CUtensorMap* map, const void* src, int x, int y, int z,
+                                               int* err = nullptr) {
+  if (!bounds_ok((x & 3) == 0 && x >= 0 && y >= 0 && z >= 0 && (smem_u32(src) & 127u) == 0, err)) return;
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
+// At most one committed bulk group of this thread is still reading its shared memory.
+__device__ __forceinline__ void bulk_wait_read_keep1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // Every committed bulk group of this thread has finished reading its shared memory.
@@ -401,6 +424,17 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
       "[%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y)
+      : "memory");
+}
+
+// The same from a 3-D map.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y,
+                                                 int z, int* err = nullptr) {
+  if (!bounds_ok((x & 7) == 0 && x >= 0 && y >= 0 && z >= 0 && (smem_u32(dst) & 1023u) == 0, err)) return;
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 

@@ -483,25 +483,37 @@ CUtensorMap make_tma_2d_bf16(const void* base, int64_t rows, int64_t cols, int64
   return map;
 }
 
-// ``planes`` row-major [rows, cols] bf16 matrices ``plane_ld`` elements apart, tiled by
-// (box_cols, box_rows, 1): a box never reaches into the next plane, it reads zeros there.
-CUtensorMap make_tma_3d_bf16(const void* base, int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld,
-                             int box_cols, int box_rows) {
+static CUtensorMap make_tma_3d(CUtensorMapDataType type, int size, CUtensorMapSwizzle swizzle, const void* base,
+                               int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld, int box_cols,
+                               int box_rows) {
   RESIHP_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0, "TMA base must be 16-byte aligned");
-  RESIHP_CHECK((ld * 2) % 16 == 0 && (plane_ld * 2) % 16 == 0, "TMA strides must be multiples of 16 bytes");
+  RESIHP_CHECK((ld * size) % 16 == 0 && (plane_ld * size) % 16 == 0, "TMA strides must be multiples of 16 bytes");
   int dev = 0;
   RESIHP_CUDA_CHECK(cudaGetDevice(&dev));
   RESIHP_CUDA_CHECK(cudaSetDevice(dev));  // make the context current (see make_tma_2d_bf16)
   CUtensorMap map;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * 2), static_cast<cuuint64_t>(plane_ld * 2)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * size), static_cast<cuuint64_t>(plane_ld * size)};
   cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-                           estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_fn()(&map, type, 3, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RESIHP_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", int(r));
   return map;
+}
+
+// ``planes`` row-major [rows, cols] matrices ``plane_ld`` elements apart, tiled by (box_cols,
+// box_rows, 1): a box never reaches into the next plane. bf16 with 128-byte swizzle (loads
+// read zeros past the edges), fp32 with 64-byte swizzle (box_cols = 16; stores are clipped).
+CUtensorMap make_tma_3d_bf16(const void* base, int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld,
+                             int box_cols, int box_rows) {
+  return make_tma_3d(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, base, planes, rows, cols, ld,
+                     plane_ld, box_cols, box_rows);
+}
+CUtensorMap make_tma_3d_f32(const void* base, int64_t planes, int64_t rows, int64_t cols, int box_rows) {
+  return make_tma_3d(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, CU_TENSOR_MAP_SWIZZLE_64B, base, planes, rows, cols, cols,
+                     rows * cols, 16, box_rows);
 }
 
 static int num_sms() {

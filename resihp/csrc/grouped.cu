@@ -30,8 +30,6 @@ namespace resihp {
 namespace {
 
 constexpr int kMaxGroups = kMoeMaxExperts;
-constexpr int kBM = 128;
-constexpr int kBK = 64;
 
 struct Args {
   void* c;
@@ -39,17 +37,6 @@ struct Args {
   const int* offsets;
   int groups, rows, n, k;
   int* err;
-};
-
-template <int BN>
-struct Tile {
-  static constexpr int kStages = BN == 256 ? 4 : 6;
-  static constexpr int kABytes = kBM * kBK * 2;
-  static constexpr int kBBytes = BN * kBK * 2;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kListBytes = 2 * (kMaxGroups + 2) * 4;
-  static constexpr int kSmem = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/ + kListBytes;
-  static constexpr int kTmemCols = 2 * BN;
 };
 
 // The groups' first rows and first tiles. Group ``groups`` is the rows behind the last one.
@@ -116,27 +103,52 @@ __device__ __forceinline__ int group_of(const Lists& l, int groups, int t, int f
   return lo;
 }
 
-__device__ __forceinline__ void store_bf16(const Args& g, int row, int col0, const uint32_t (&v)[32]) {
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(g.c) + int64_t(row) * g.ldc + col0;
-  #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (col0 + 8 * j >= g.n) break;
-    uint4 o;
-    o.x = pack_bf16(__uint_as_float(v[8 * j]), __uint_as_float(v[8 * j + 1]));
-    o.y = pack_bf16(__uint_as_float(v[8 * j + 2]), __uint_as_float(v[8 * j + 3]));
-    o.z = pack_bf16(__uint_as_float(v[8 * j + 4]), __uint_as_float(v[8 * j + 5]));
-    o.w = pack_bf16(__uint_as_float(v[8 * j + 6]), __uint_as_float(v[8 * j + 7]));
-    *reinterpret_cast<uint4*>(out + 8 * j) = o;
-  }
+// ---- rows: forward and input gradient --------------------------------------------------
+//
+// The product is computed transposed, c^T = w a^T: the weights' output features are the MMA's
+// M (256 per CTA pair, 128 per CTA), the group's rows its N. N is an operand of each MMA, a
+// multiple of 32 up to TN, so a group whose length is no multiple of a tile costs what its
+// rows cost (at 8 groups of about 1024 rows, 256-row M tiles would do 12 % more work), and a
+// handful of rows costs one narrow MMA per K step while the weights stream past. A group of
+// more than TN rows is cut into equal parts, not into full tiles and a rest.
+
+constexpr int kBK = 64;
+
+template <int TN>
+struct RowTile {
+  static constexpr int kWBytes = 128 * kBK * 2;         // this CTA's 128 features
+  static constexpr int kABytes = TN / 2 * kBK * 2;      // this CTA's half of the rows
+  static constexpr int kStageBytes = kWBytes + kABytes;
+  static constexpr int kStages = TN == 256 ? 6 : 10;
+  static constexpr int kListBytes = 2 * (kMaxGroups + 2) * 4;
+  static constexpr int kSmem = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/ + kListBytes;
+  static constexpr int kTmemCols = 2 * TN;
+  static_assert(kSmem <= 232448, "grouped stages exceed the shared memory of a CTA");
+  static_assert((2 * kStages + 4) * 8 + 4 <= 256, "grouped barriers exceed their area");
+};
+
+// Rows of a tile as the pair MMA takes them: its N goes in steps of 32.
+__device__ __forceinline__ int mma_rows(int rows) { return (rows + 31) & ~31; }
+
+struct RowSpan {
+  int row0, rows, f0;  // first row, row count and first output feature of a tile
+};
+
+template <int TN>
+__device__ __forceinline__ RowSpan span_of(const Lists& l, int e, int t, int tiles_f) {
+  const int size = l.row[e + 1] - l.row[e];
+  const int parts = (l.tile[e + 1] - l.tile[e]) / tiles_f;
+  int tm, tf;
+  tile_coords(t - l.tile[e], parts, tiles_f, tm, tf);
+  const int each = mma_rows((size + parts - 1) / parts);  // parts * each >= size, each <= TN
+  return RowSpan{l.row[e] + tm * each, min(each, size - tm * each), tf * 256};
 }
 
-// ---- rows: forward and input gradient --------------------------------------------------
-
-template <int BN, bool W_MN>
+template <int TN, bool W_MN>
 __global__ void __launch_bounds__(192, 1)
-    grouped_rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w, Args g) {
+    grouped_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_a, Args g) {
   pdl_enter();
-  using S = Tile<BN>;
+  using S = RowTile<TN>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -152,7 +164,9 @@ __global__ void __launch_bounds__(192, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int tiles_n = (g.n + BN - 1) / BN;
+  const uint32_t cta = cluster_ctarank();  // 0: leader, 1: peer
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles_f = (g.n + 255) / 256;
   const int kblocks = (g.k + kBK - 1) / kBK;
 
   if (threadIdx.x == 0) {
@@ -162,16 +176,16 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 4);
+      mbar_init(&acc_empty[a], 8);
     }
     fence_barrier_init();
-    tma_prefetch(&tma_a);
     tma_prefetch(&tma_w);
+    tma_prefetch(&tma_a);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, S::kTmemCols);
-  build_lists(l, g, kBM, tiles_n);
+  if (warp == 1) tmem_alloc_pair(tmem_slot, S::kTmemCols);
+  build_lists(l, g, TN, tiles_f);
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();  // both CTAs' barriers initialised and TMEM allocated before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int work = l.tile[g.groups];        // tiles with a product
@@ -182,142 +196,190 @@ __global__ void __launch_bounds__(192, 1)
       int s = 0, e = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < work && ok; t += gridDim.x) {
+      for (int t = pair; t < work && ok; t += pairs) {
         e = group_of(l, g.groups, t, e);
-        int tm, tn;
-        tile_coords(t - l.tile[e], (l.tile[e + 1] - l.tile[e]) / tiles_n, tiles_n, tm, tn);
-        const int m0 = l.row[e] + tm * kBM, n0 = tn * BN;
+        const RowSpan p = span_of<TN>(l, e, t, tiles_f);
+        // each CTA brings its features and its half of the MMA's N rows
+        const int f0 = p.f0 + int(cta) * 128, r0 = p.row0 + int(cta) * (mma_rows(p.rows) >> 1);
         for (int kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) { ok = false; break; }
-          uint8_t* sa = smem + s * S::kStageBytes;
-          uint8_t* sb = sa + S::kABytes;
-          mbar_expect_tx(&full[s], S::kStageBytes);
+          uint8_t* sw = smem + s * S::kStageBytes;
+          uint8_t* sa = sw + S::kWBytes;
+          if (cta == 0) mbar_expect_tx(&full[s], 2 * S::kStageBytes);  // both CTAs' parts
+          const uint32_t bar = mapa_shared(&full[s], 0);
           const int k0 = kb * kBK;
-          tma_load_2d(sa, &tma_a, &full[s], k0, m0, g.err);
           if (W_MN) {
-            #pragma unroll
-            for (int c = 0; c < BN / 64; ++c) tma_load_3d(sb + c * 8192, &tma_w, &full[s], n0 + 64 * c, k0, e, g.err);
+            tma_load_3d_pair(sw, &tma_w, bar, f0, k0, e, g.err);
+            tma_load_3d_pair(sw + 8192, &tma_w, bar, f0 + 64, k0, e, g.err);
           } else {
-            tma_load_3d(sb, &tma_w, &full[s], k0, n0, e, g.err);
+            tma_load_3d_pair(sw, &tma_w, bar, k0, f0, e, g.err);
           }
+          tma_load_2d_pair(sa, &tma_a, bar, k0, r0, g.err);
           if (++s == kStages) { s = 0; ph ^= 1; }
         }
       }
+      // Producer tail: wait until the leader has released every stage, so no pair-MMA
+      // commit can arrive on this CTA's barriers after it exits.
+      for (int j = 0; j < kStages && ok; ++j) {
+        if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) break;
+        if (++s == kStages) { s = 0; ph ^= 1; }
+      }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16_f32(kBM, BN, 0, W_MN ? 1 : 0);
-      int s = 0, i = 0;
+    if (cta == 0 && lane == 0) {
+      int s = 0, i = 0, e = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < work && ok; t += gridDim.x, ++i) {
+      for (int t = pair; t < work && ok; t += pairs, ++i) {
+        e = group_of(l, g.groups, t, e);
+        const RowSpan p = span_of<TN>(l, e, t, tiles_f);
+        const uint32_t idesc = idesc_bf16_f32(256, mma_rows(p.rows), W_MN ? 1 : 0, 0);
         const int a = i & 1;
-        if (!mbar_wait(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait)) break;
+        if (!mbar_wait_cluster(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait)) break;
         tc_fence_after();
-        const uint32_t d = tmem_base + a * BN;
-        if (!tmem_span_ok(d, tmem_base, S::kTmemCols, BN, g.err)) break;
+        const uint32_t d = tmem_base + a * TN;
+        if (!tmem_span_ok(d, tmem_base, S::kTmemCols, mma_rows(p.rows), g.err)) break;
         for (int kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait(&full[s], ph, g.err, kErrMmaWait)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * S::kStageBytes);
-          const uint32_t sb = sa + S::kABytes;
+          const uint32_t sw = smem_u32(smem + s * S::kStageBytes);
+          const uint32_t sa = sw + S::kWBytes;
           #pragma unroll
           for (int kk = 0; kk < kBK / 16; ++kk) {
-            const uint64_t da = smem_desc_sw128(sa + kk * 32, 16, 1024);
-            const uint64_t db = W_MN ? smem_desc_sw128(sb + kk * 2048, 8192, 1024)
-                                     : smem_desc_sw128(sb + kk * 32, 16, 1024);
-            umma_bf16(d, da, db, idesc, (kb | kk) != 0);
+            const uint64_t dw = W_MN ? smem_desc_sw128(sw + kk * 2048, 8192, 1024)
+                                     : smem_desc_sw128(sw + kk * 32, 16, 1024);
+            umma_bf16_pair(d, dw, smem_desc_sw128(sa + kk * 32, 16, 1024), idesc, (kb | kk) != 0);
           }
-          umma_commit(&empty[s]);
+          umma_commit_pair(smem_u32(&empty[s]));
+          umma_commit_pair(mapa_shared(&empty[s], 1));
           if (++s == kStages) { s = 0; ph ^= 1; }
         }
-        umma_commit(&acc_full[a]);
+        if (!ok) break;
+        umma_commit_pair(smem_u32(&acc_full[a]));
+        umma_commit_pair(mapa_shared(&acc_full[a], 1));
       }
     }
   } else {
     const int q = warp & 3;  // TMEM lane quarter this warp may access
+    const uint32_t acc_empty_leader0 = mapa_shared(&acc_empty[0], 0);
+    const uint32_t acc_empty_leader1 = mapa_shared(&acc_empty[1], 0);
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(g.c);
     int i = 0, e = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+    for (int t = pair; t < tiles; t += pairs, ++i) {
       e = group_of(l, g.groups, t, e);
-      int tm, tn;
-      tile_coords(t - l.tile[e], (l.tile[e + 1] - l.tile[e]) / tiles_n, tiles_n, tm, tn);
-      const int row = l.row[e] + tm * kBM + q * 32 + lane;
-      const bool row_ok = row < l.row[e + 1];
-      if (e == g.groups) {  // behind the last group: zeros
-        const uint32_t zero[32] = {};
-        for (int c = 0; c < BN / 32; ++c)
-          if (row_ok && tn * BN + c * 32 < g.n) store_bf16(g, row, tn * BN + c * 32, zero);
+      const RowSpan p = span_of<TN>(l, e, t, tiles_f);
+      const int fc = p.f0 + int(cta) * 128;  // this CTA's first feature
+      if (e == g.groups) {  // behind the last group: zeros, 128 features of a row per half warp
+        const int f = fc + (lane & 15) * 8;
+        for (int r = q * 2 + (lane >> 4); r < p.rows; r += 8)
+          if (f < g.n) *reinterpret_cast<uint4*>(out + int64_t(p.row0 + r) * g.ldc + f) = make_uint4(0, 0, 0, 0);
         continue;
       }
       const int a = i & 1;
       if (!mbar_wait(&acc_full[a], (i >> 1) & 1, g.err, kErrEpiWait)) break;
       tc_fence_after();
+      // Lane f holds feature f of 32 rows. Neighbouring lanes swap one value per two rows, so
+      // that each stores two features of one row: a warp's store covers 64 bytes of two rows.
+      const int f = fc + q * 32 + (lane & ~1);
+      const bool odd = lane & 1;
+      __nv_bfloat16* base = out + int64_t(p.row0 + (odd ? 1 : 0)) * g.ldc + f;
       #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
+      for (int c = 0; c < p.rows; c += 32) {
         uint32_t v[32];
-        const uint32_t ta = tmem_base + a * BN + c * 32 + (uint32_t(q * 32) << 16);
+        const uint32_t ta = tmem_base + a * TN + c + (uint32_t(q * 32) << 16);
         if (!tmem_span_ok(ta, tmem_base, S::kTmemCols, 32, g.err)) continue;
         tmem_ld32(ta, v);
         tmem_wait_ld();
-        const int col0 = tn * BN + c * 32;
-        if (row_ok && col0 < g.n) store_bf16(g, row, col0, v);
+        #pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
+          const uint32_t o = odd ? pack_bf16(__uint_as_float(got), __uint_as_float(v[j + 1]))
+                                 : pack_bf16(__uint_as_float(v[j]), __uint_as_float(got));
+          if (c + j + (odd ? 1 : 0) < p.rows && f < g.n)
+            *reinterpret_cast<uint32_t*>(base + int64_t(c + j) * g.ldc) = o;
+        }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[a]);
+      if (lane == 0) mbar_arrive_remote(a == 0 ? acc_empty_leader0 : acc_empty_leader1);
     }
   }
 
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();  // no CTA leaves while its pair may still touch its barriers or TMEM
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, S::kTmemCols);
+    tmem_dealloc_pair(tmem_base, S::kTmemCols);
   }
 }
 
 // ---- weight gradient --------------------------------------------------------------------
+//
+// Tile: 128 output features (n) x 256 input features (k) of one group, reduced over its rows
+// in blocks of 32. The tensor cores add into an accumulator with truncation, so a long sum
+// drifts (2e-6 of its norm per 1024 rows, growing with the length); every 256 rows the
+// accumulator is therefore handed to the epilogue, which adds it to fp32 registers with
+// rounding, while the MMAs go on in the other accumulator. Eight epilogue warps keep 128
+// columns of a row per thread. The finished tile leaves through shared memory as bulk
+// stores or bulk additions (whole 64-byte runs, clipped at the matrix's edges by the map):
+// each element is added to once per launch, so the sum does not depend on any order.
 
-// Tile rows are the group's output features (n), tile columns its input features (k).
-template <int BN, bool ACC>
-__global__ void __launch_bounds__(192, 1)
-    grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tma_dy, const __grid_constant__ CUtensorMap tma_x, Args g) {
+constexpr int kWK = 32;          // rows per block
+constexpr int kWChunk = 8;       // blocks per accumulator
+constexpr int kWStages = 7;
+constexpr int kWThreads = 320;   // producer, MMA, eight epilogue warps
+struct WgradTile {
+  static constexpr int kChunkBytes = 64 * kWK * 2;  // 64 columns of a block, MN-major
+  static constexpr int kABytes = 2 * kChunkBytes;
+  static constexpr int kStageBytes = 6 * kChunkBytes;
+  static constexpr int kOutBytes = 2 * 32 * 16 * 4;  // per epilogue warp: two 32 x 16 fp32 buffers
+  static constexpr int kListBytes = 2 * (kMaxGroups + 2) * 4;
+  static constexpr int kSmem = kWStages * kStageBytes + 8 * kOutBytes + 1024 + 256 + kListBytes;
+  static constexpr int kTmemCols = 512;
+  static_assert(kSmem <= 232448, "grouped wgrad stages exceed the shared memory of a CTA");
+};
+
+template <bool ACC>
+__global__ void __launch_bounds__(kWThreads, 1)
+    grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tma_dy, const __grid_constant__ CUtensorMap tma_x,
+                         const __grid_constant__ CUtensorMap tma_c, Args g) {
   pdl_enter();
-  using S = Tile<BN>;
-  constexpr int kStages = S::kStages;
+  using S = WgradTile;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024 - (raw & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * S::kStageBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
+  uint8_t* staging = smem + kWStages * S::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * S::kOutBytes);
+  uint64_t* empty = full + kWStages;
+  uint64_t* acc_full = empty + kWStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   Lists l;
-  l.row = reinterpret_cast<int*>(smem + kStages * S::kStageBytes + 256);
+  l.row = reinterpret_cast<int*>(staging + 8 * S::kOutBytes + 256);
   l.tile = l.row + kMaxGroups + 2;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int tiles_m = (g.n + kBM - 1) / kBM, tiles_n = (g.k + BN - 1) / BN;
+  const int tiles_m = (g.n + 127) / 128, tiles_n = (g.k + 255) / 256;
   const int per_group = tiles_m * tiles_n;
   const int tiles = g.groups * per_group;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kWStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 4);
+      mbar_init(&acc_empty[a], 8);
     }
     fence_barrier_init();
     tma_prefetch(&tma_dy);
     tma_prefetch(&tma_x);
+    tma_prefetch(&tma_c);
   }
   if (warp == 1) tmem_alloc(tmem_slot, S::kTmemCols);
-  build_lists(l, g, kBK, 1);  // "tiles": the group's K blocks
+  build_lists(l, g, kWK, 1);  // "tiles": the group's row blocks
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -332,116 +394,128 @@ __global__ void __launch_bounds__(192, 1)
         const int e = t / per_group;
         int tm, tn;
         tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
-        const int kblocks = l.tile[e + 1] - l.tile[e];
-        const int m0 = tm * kBM, n0 = tn * BN;
-        for (int kb = 0; kb < kblocks; ++kb) {
+        const int blocks = l.tile[e + 1] - l.tile[e];
+        const int m0 = tm * 128, n0 = tn * 256;
+        for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) { ok = false; break; }
           uint8_t* sa = smem + s * S::kStageBytes;
           uint8_t* sb = sa + S::kABytes;
           mbar_expect_tx(&full[s], S::kStageBytes);
-          const int r0 = l.row[e] + kb * kBK;
+          const int r0 = l.row[e] + kb * kWK;
           #pragma unroll
-          for (int c = 0; c < kBM / 64; ++c) tma_load_2d(sa + c * 8192, &tma_dy, &full[s], m0 + 64 * c, r0, g.err);
+          for (int c = 0; c < 2; ++c) tma_load_2d(sa + c * S::kChunkBytes, &tma_dy, &full[s], m0 + 64 * c, r0, g.err);
           #pragma unroll
-          for (int c = 0; c < BN / 64; ++c) tma_load_2d(sb + c * 8192, &tma_x, &full[s], n0 + 64 * c, r0, g.err);
-          if (++s == kStages) { s = 0; ph ^= 1; }
+          for (int c = 0; c < 4; ++c) tma_load_2d(sb + c * S::kChunkBytes, &tma_x, &full[s], n0 + 64 * c, r0, g.err);
+          if (++s == kWStages) { s = 0; ph ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
-    // the whole warp walks the stages (it zeroes a cut K block together); lane 0 issues
-    constexpr uint32_t idesc = idesc_bf16_f32(kBM, BN, 1, 1);
+    // the whole warp walks the stages (it zeroes a cut block together); lane 0 issues
+    constexpr uint32_t idesc = idesc_bf16_f32(128, 256, 1, 1);
     int s = 0, i = 0;
     uint32_t ph = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const int e = t / per_group;
-      const int kblocks = l.tile[e + 1] - l.tile[e];
-      if (kblocks == 0) continue;
       const int size = l.row[e + 1] - l.row[e];
-      const int a = i & 1;
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait))) break;
-      ++i;
-      tc_fence_after();
-      const uint32_t d = tmem_base + a * BN;
-      if (!tmem_span_ok(d, tmem_base, S::kTmemCols, BN, g.err)) break;
-      for (int kb = 0; kb < kblocks; ++kb) {
+      const int blocks = l.tile[e + 1] - l.tile[e];
+      for (int kb = 0; kb < blocks; ++kb) {
+        const int a = i & 1;
+        const uint32_t d = tmem_base + a * 256;
+        if (kb % kWChunk == 0) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait))) { ok = false; break; }
+          tc_fence_after();
+        }
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[s], ph, g.err, kErrMmaWait))) { ok = false; break; }
-        const int valid = min(kBK, size - kb * kBK);
+        const int valid = min(kWK, size - kb * kWK);
         const int steps = (valid + 15) / 16;
-        uint8_t* sa_p = smem + s * S::kStageBytes;
+        uint8_t* stage = smem + s * S::kStageBytes;
         if (valid < 16 * steps) {
-          // MN-major chunks are 64 rows of 128 bytes: rows valid .. 16 * steps hold the
-          // next group's rows (both operands: 0 * inf would not be 0)
+          // MN-major chunks are rows of 128 bytes: rows valid .. 16 * steps hold the next
+          // group's rows (zeroed in both operands: 0 * inf would not be 0)
           const int bytes = (16 * steps - valid) * 128;
           #pragma unroll 1
-          for (int c = 0; c < (kBM + BN) / 64; ++c)
+          for (int c = 0; c < 6; ++c)
             for (int b = lane * 16; b < bytes; b += 512)
-              *reinterpret_cast<uint4*>(sa_p + c * 8192 + valid * 128 + b) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(stage + c * S::kChunkBytes + valid * 128 + b) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
           __syncwarp();
         }
         if (lane == 0) {
           tc_fence_after();
-          const uint32_t sa = smem_u32(sa_p);
+          const uint32_t sa = smem_u32(stage);
           const uint32_t sb = sa + S::kABytes;
           for (int kk = 0; kk < steps; ++kk)
-            umma_bf16(d, smem_desc_sw128(sa + kk * 2048, 8192, 1024), smem_desc_sw128(sb + kk * 2048, 8192, 1024),
-                      idesc, (kb | kk) != 0);
+            umma_bf16(d, smem_desc_sw128(sa + kk * 2048, S::kChunkBytes, 1024),
+                      smem_desc_sw128(sb + kk * 2048, S::kChunkBytes, 1024), idesc, kb % kWChunk != 0 || kk != 0);
           umma_commit(&empty[s]);
         }
         __syncwarp();
-        if (++s == kStages) { s = 0; ph ^= 1; }
+        if (++s == kWStages) { s = 0; ph ^= 1; }
+        if (kb % kWChunk == kWChunk - 1 || kb == blocks - 1) {
+          if (lane == 0) umma_commit(&acc_full[a]);
+          __syncwarp();
+          ++i;
+        }
       }
-      if (lane == 0) umma_commit(&acc_full[a]);
-      __syncwarp();
     }
   } else {
-    const int q = warp & 3;
-    int i = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int q = warp & 3;           // TMEM lane quarter this warp may access
+    const int half = (warp - 2) >> 2;  // columns 128 * half .. + 127 of the tile
+    uint8_t* buf = staging + (warp - 2) * S::kOutBytes;
+    int i = 0, turn = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const int e = t / per_group;
-      const bool empty_group = l.tile[e + 1] == l.tile[e];
-      if (empty_group && ACC) continue;
-      int tm, tn;
-      tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
-      const int row = tm * kBM + q * 32 + lane;
-      const bool row_ok = row < g.n;
-      float* out = static_cast<float*>(g.c) + (int64_t(e) * g.n + row) * g.k;
-      const int a = i & 1;
-      if (!empty_group) {
-        if (!mbar_wait(&acc_full[a], (i >> 1) & 1, g.err, kErrEpiWait)) break;
-        ++i;
+      const int blocks = l.tile[e + 1] - l.tile[e];
+      if (blocks == 0 && ACC) continue;
+      float acc[128];
+      #pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      for (int c = 0; c < blocks; c += kWChunk, ++i) {
+        const int a = i & 1;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[a], (i >> 1) & 1, g.err, kErrEpiWait))) { ok = false; break; }
         tc_fence_after();
-      }
-      #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
-        uint32_t v[32];
-        if (empty_group) {
-          #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0u;
-        } else {
-          const uint32_t ta = tmem_base + a * BN + c * 32 + (uint32_t(q * 32) << 16);
-          if (!tmem_span_ok(ta, tmem_base, S::kTmemCols, 32, g.err)) continue;
-          tmem_ld32(ta, v);
-          tmem_wait_ld();
-        }
-        const int col0 = tn * BN + c * 32;
         #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (!row_ok || col0 + 4 * j >= g.k) break;
-          const float4 o = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
-                                       __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
-          if (ACC) red_add_v4(out + col0 + 4 * j, o);
-          else *reinterpret_cast<float4*>(out + col0 + 4 * j) = o;
+          uint32_t v[16];
+          tmem_ld16(tmem_base + a * 256 + half * 128 + j * 16 + (uint32_t(q * 32) << 16), v);
+          tmem_wait_ld();
+          #pragma unroll
+          for (int x = 0; x < 16; ++x) acc[j * 16 + x] += __uint_as_float(v[x]);
         }
-      }
-      if (!empty_group) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[a]);
       }
+      if (!ok) break;
+      int tm, tn;
+      tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
+      const int row0 = tm * 128 + q * 32, col0 = tn * 256 + half * 128;
+      if (row0 >= g.n) continue;
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) {  // 16 columns at a time through one of two buffers
+        if (col0 + j * 16 < g.k) {
+          if (lane == 0) bulk_wait_read_keep1();
+          __syncwarp();
+          uint8_t* b = buf + turn * (S::kOutBytes / 2);
+          #pragma unroll
+          for (int x = 0; x < 4; ++x)  // the map's 64-byte swizzle: 16-byte unit x of row r is at x ^ (r / 2) % 4
+            *reinterpret_cast<float4*>(b + lane * 64 + ((x ^ ((lane >> 1) & 3)) << 4)) =
+                make_float4(acc[j * 16 + 4 * x], acc[j * 16 + 4 * x + 1], acc[j * 16 + 4 * x + 2], acc[j * 16 + 4 * x + 3]);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if (ACC) tma_add_3d_f32(&tma_c, b, col0 + j * 16, row0, e, g.err);
+            else tma_store_3d_f32(&tma_c, b, col0 + j * 16, row0, e, g.err);
+            bulk_commit();
+          }
+          turn ^= 1;
+        }
+      }
     }
+    if (lane == 0) bulk_wait_all();
   }
 
   tc_fence_before();
@@ -462,12 +536,52 @@ int num_sms() {
   return counts[dev];
 }
 
-template <typename Kernel>
-void launch(Kernel kernel, int smem, int64_t tiles, const CUtensorMap& ta, const CUtensorMap& tb, const Args& g,
-            cudaStream_t st) {
-  RESIHP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int grid = int(std::min<int64_t>(tiles, num_sms()));
-  RESIHP_CUDA_CHECK(launch_pdl(kernel, grid, 192, smem, st, ta, tb, g));
+// Pairs of CTAs that can be resident at once (a persistent grid larger than that only queues).
+template <int TN, bool W_MN>
+void launch_rows(int64_t tiles, const CUtensorMap& tw, const CUtensorMap& ta, const Args& g, cudaStream_t st) {
+  auto kernel = grouped_rows_kernel<TN, W_MN>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel starts with pdl_enter()
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.blockDim = dim3(192, 1, 1);
+  cfg.dynamicSmemBytes = RowTile<TN>::kSmem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  static int resident[64] = {0};
+  int dev = 0;
+  RESIHP_CUDA_CHECK(cudaGetDevice(&dev));
+  if (resident[dev] == 0) {
+    RESIHP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowTile<TN>::kSmem));
+    cfg.gridDim = dim3(2, 1, 1);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = num_sms() / 2;
+    }
+    resident[dev] = n;
+  }
+  cfg.gridDim = dim3(2 * unsigned(std::min<int64_t>(tiles, resident[dev])), 1, 1);
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  RESIHP_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, tw, ta, g));
+}
+
+template <int TN>
+void launch_rows_tn(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t w_group, bool w_mn,
+                    const GroupedShape& s, const Args& g, cudaStream_t st) {
+  const int64_t tiles_f = (s.n + 255) / 256;
+  const int64_t most = (int64_t(s.rows) + TN - 1) / TN + s.groups + 1;  // row tiles, if every group cuts one
+  RESIHP_CHECK(most * tiles_f <= INT32_MAX, "grouped products: too many tiles");
+  const CUtensorMap ta = make_tma_2d_bf16(a, s.rows, s.k, lda, 64, TN / 2);
+  const CUtensorMap tw = w_mn ? make_tma_3d_bf16(w, s.groups, s.k, s.n, ldw, w_group, 64, 64)
+                              : make_tma_3d_bf16(w, s.groups, s.n, s.k, ldw, w_group, 64, 128);
+  if (w_mn) launch_rows<TN, true>(most * tiles_f, tw, ta, g, st);
+  else launch_rows<TN, false>(most * tiles_f, tw, ta, g, st);
 }
 
 void check_shape(const GroupedShape& s) {
@@ -484,17 +598,10 @@ void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_
   check_shape(s);
   if (s.rows == 0) return;
   RESIHP_CHECK(reinterpret_cast<uintptr_t>(c) % 16 == 0 && ldc % 8 == 0, "grouped output must be 16-byte aligned");
-  constexpr int BN = 128;
-  const int64_t tiles_n = (s.n + BN - 1) / BN;
-  const int64_t most = (int64_t(s.rows) + kBM - 1) / kBM + s.groups + 1;  // tile rows, if every group cuts one
-  RESIHP_CHECK(most * tiles_n <= INT32_MAX, "grouped products: too many tiles");
-  const CUtensorMap ta = make_tma_2d_bf16(a, s.rows, s.k, lda, 64, kBM);
-  const CUtensorMap tw = w_mn ? make_tma_3d_bf16(w, s.groups, s.k, s.n, ldw, w_group, 64, 64)
-                              : make_tma_3d_bf16(w, s.groups, s.n, s.k, ldw, w_group, 64, BN);
   const Args g{c, ldc, s.offsets, s.groups, s.rows, s.n, s.k, err};
-  using S = Tile<BN>;
-  if (w_mn) launch(grouped_rows_kernel<BN, true>, S::kSmem, most * tiles_n, ta, tw, g, st);
-  else launch(grouped_rows_kernel<BN, false>, S::kSmem, most * tiles_n, ta, tw, g, st);
+  // Few rows per group: narrow row tiles, whose smaller stages keep ten weight tiles in flight.
+  if (s.rows <= int64_t(48) * s.groups) launch_rows_tn<64>(a, lda, w, ldw, w_group, w_mn, s, g, st);
+  else launch_rows_tn<256>(a, lda, w, ldw, w_group, w_mn, s, g, st);
 }
 
 void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, float* c, bool accumulate,
@@ -505,15 +612,16 @@ void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, flo
     if (!accumulate) RESIHP_CUDA_CHECK(cudaMemsetAsync(c, 0, sizeof(float) * size_t(s.groups) * s.n * s.k, st));
     return;
   }
-  constexpr int BN = 128;
-  const int64_t tiles = int64_t(s.groups) * ((s.n + kBM - 1) / kBM) * ((s.k + BN - 1) / BN);
+  const int64_t tiles = int64_t(s.groups) * ((s.n + 127) / 128) * ((s.k + 255) / 256);
   RESIHP_CHECK(tiles <= INT32_MAX, "grouped products: too many tiles");
-  const CUtensorMap ta = make_tma_2d_bf16(dy, s.rows, s.n, lddy, 64, 64);
-  const CUtensorMap tb = make_tma_2d_bf16(x, s.rows, s.k, ldx, 64, 64);
+  const CUtensorMap ta = make_tma_2d_bf16(dy, s.rows, s.n, lddy, 64, kWK);
+  const CUtensorMap tb = make_tma_2d_bf16(x, s.rows, s.k, ldx, 64, kWK);
+  const CUtensorMap tc = make_tma_3d_f32(c, s.groups, s.n, s.k, 32);
   const Args g{c, 0, s.offsets, s.groups, s.rows, s.n, s.k, err};
-  using S = Tile<BN>;
-  if (accumulate) launch(grouped_wgrad_kernel<BN, true>, S::kSmem, tiles, ta, tb, g, st);
-  else launch(grouped_wgrad_kernel<BN, false>, S::kSmem, tiles, ta, tb, g, st);
+  auto kernel = accumulate ? grouped_wgrad_kernel<true> : grouped_wgrad_kernel<false>;
+  RESIHP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WgradTile::kSmem));
+  const int grid = int(std::min<int64_t>(tiles, num_sms()));
+  RESIHP_CUDA_CHECK(launch_pdl(kernel, grid, kWThreads, WgradTile::kSmem, st, ta, tb, tc, g));
 }
 
 }  // namespace resihp

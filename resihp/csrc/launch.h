@@ -218,5 +218,6 @@ void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, flo
                    const GroupedShape& s, int* err, cudaStream_t st);
 CUtensorMap make_tma_3d_bf16(const void* base, int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld,
                              int box_cols, int box_rows);
+CUtensorMap make_tma_3d_f32(const void* base, int64_t planes, int64_t rows, int64_t cols, int box_rows);
 
 }  // namespace resihp
