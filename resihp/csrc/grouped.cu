@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(192, 1)
   l.row = reinterpret_cast<int*>(smem + kStages * S::kStageBytes + 256);
   l.tile = l.row + kMaxGroups + 2;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0);  // uniform for the compiler too
   const int lane = threadIdx.x & 31;
   const uint32_t cta = cluster_ctarank();  // 0: leader, 1: peer
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -226,37 +226,39 @@ __global__ void __launch_bounds__(192, 1)
       }
     }
   } else if (warp == 1) {
-    if (cta == 0 && lane == 0) {
+    if (cta == 0) {  // the whole warp walks, one lane issues
+      const uint32_t issue = elect_one();
+      const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(empty), bar1 = mapa_shared(empty, 1);
+      const uint32_t done0 = smem_u32(acc_full), done1 = mapa_shared(acc_full, 1);
       int s = 0, i = 0, e = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int t = pair; t < work && ok; t += pairs, ++i) {
         e = group_of(l, g.groups, t, e);
-        const RowSpan p = span_of<TN>(l, e, t, tiles_f);
-        const uint32_t idesc = idesc_bf16_f32(256, mma_rows(p.rows), W_MN ? 1 : 0, 0);
+        const int n = __shfl_sync(0xFFFFFFFFu, mma_rows(span_of<TN>(l, e, t, tiles_f).rows), 0);
+        const uint32_t idesc = idesc_bf16_f32(256, n, W_MN ? 1 : 0, 0);
         const int a = i & 1;
-        if (!mbar_wait_cluster(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait)) break;
-        tc_fence_after();
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait))) break;
         const uint32_t d = tmem_base + a * TN;
-        if (!tmem_span_ok(d, tmem_base, S::kTmemCols, mma_rows(p.rows), g.err)) break;
+        if (!tmem_span_ok(d, tmem_base, S::kTmemCols, n, g.err)) break;
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&full[s], ph, g.err, kErrMmaWait)) { ok = false; break; }
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[s], ph, g.err, kErrMmaWait))) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sw = smem_u32(smem + s * S::kStageBytes);
-          const uint32_t sa = sw + S::kWBytes;
+          // the descriptors' address field counts 16-byte units: a K step adds to it
+          const uint32_t sw = sbase + s * S::kStageBytes;
+          const uint64_t dw = W_MN ? smem_desc_sw128(sw, 8192, 1024) : smem_desc_sw128(sw, 16, 1024);
+          const uint64_t da = smem_desc_sw128(sw + S::kWBytes, 16, 1024);
           #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            const uint64_t dw = W_MN ? smem_desc_sw128(sw + kk * 2048, 8192, 1024)
-                                     : smem_desc_sw128(sw + kk * 32, 16, 1024);
-            umma_bf16_pair(d, dw, smem_desc_sw128(sa + kk * 32, 16, 1024), idesc, (kb | kk) != 0);
-          }
-          umma_commit_pair(smem_u32(&empty[s]));
-          umma_commit_pair(mapa_shared(&empty[s], 1));
+          for (int kk = 0; kk < kBK / 16; ++kk)
+            umma_bf16_pair_if(issue, d, dw + kk * (W_MN ? 2048 / 16 : 32 / 16), da + kk * (32 / 16), idesc,
+                              (kb | kk) != 0);
+          umma_commit_pair_if(issue, bar0 + s * 8);
+          umma_commit_pair_if(issue, bar1 + s * 8);
           if (++s == kStages) { s = 0; ph ^= 1; }
         }
         if (!ok) break;
-        umma_commit_pair(smem_u32(&acc_full[a]));
-        umma_commit_pair(mapa_shared(&acc_full[a], 1));
+        umma_commit_pair_if(issue, done0 + a * 8);
+        umma_commit_pair_if(issue, done1 + a * 8);
       }
     }
   } else {
@@ -315,29 +317,40 @@ __global__ void __launch_bounds__(192, 1)
 
 // ---- weight gradient --------------------------------------------------------------------
 //
-// Tile: 128 output features (n) x 256 input features (k) of one group, reduced over its rows
-// in blocks of 32. The tensor cores add into an accumulator with truncation, so a long sum
-// drifts (2e-6 of its norm per 1024 rows, growing with the length); every 256 rows the
-// accumulator is therefore handed to the epilogue, which adds it to fp32 registers with
-// rounding, while the MMAs go on in the other accumulator. Eight epilogue warps keep 128
-// columns of a row per thread. The finished tile leaves through shared memory as bulk
-// stores or bulk additions (whole 64-byte runs, clipped at the matrix's edges by the map):
-// each element is added to once per launch, so the sum does not depend on any order.
+// Tile: 256 output features (n) x 256 input features (k) of one group on a CTA pair, reduced
+// over the group's rows in blocks of 64. The tensor cores add into an accumulator with
+// truncation, so a long sum drifts: off by 1e-6 of its norm after 1024 rows, 4e-6 after 4096,
+// 1.9e-5 after 16384 (an fp32 library product: 3e-7 to 6e-7). Every 512 rows the accumulator is
+// therefore handed to the epilogue, which adds it to fp32 registers with rounding, while the
+// MMAs go on in the other accumulator: 4.8e-7 at every length, for 3 % of the rate (1222
+// against 1255 TF/s, two groups of 8192 rows; every 256 rows 2.7e-7 at 1125). Eight epilogue
+// warps per CTA keep 128 columns of a row per thread. The finished tile leaves through shared
+// memory as bulk stores or bulk additions (whole 64-byte runs, clipped at the matrix's edges
+// by the map): each element is added to once per launch, so no order can change the sum.
+//
+// A group's last block holds rows of the next group where its length is no multiple of 64.
+// Steps of 16 rows past the end are not issued; rows past the end inside the last step are
+// zeroed in shared memory by warp 2 of each CTA. Such a block's loads complete on the CTA's own
+// ``cut`` barrier, and the leader's MMAs wait for both CTAs' arrivals on ``zeroed``.
 
-constexpr int kWK = 32;          // rows per block
 constexpr int kWChunk = 8;       // blocks per accumulator
-constexpr int kWStages = 7;
-constexpr int kWThreads = 320;   // producer, MMA, eight epilogue warps
+constexpr int kWStages = 5;
+constexpr int kWThreads = 352;   // producer, MMA, zeroing, eight epilogue warps
 struct WgradTile {
-  static constexpr int kChunkBytes = 64 * kWK * 2;  // 64 columns of a block, MN-major
-  static constexpr int kABytes = 2 * kChunkBytes;
-  static constexpr int kStageBytes = 6 * kChunkBytes;
+  static constexpr int kChunkBytes = 64 * kBK * 2;  // 64 columns of a block, MN-major
+  static constexpr int kABytes = 2 * kChunkBytes;   // this CTA's 128 columns of dy, then of x
+  static constexpr int kStageBytes = 4 * kChunkBytes;
   static constexpr int kOutBytes = 2 * 32 * 16 * 4;  // per epilogue warp: two 32 x 16 fp32 buffers
   static constexpr int kListBytes = 2 * (kMaxGroups + 2) * 4;
   static constexpr int kSmem = kWStages * kStageBytes + 8 * kOutBytes + 1024 + 256 + kListBytes;
   static constexpr int kTmemCols = 512;
   static_assert(kSmem <= 232448, "grouped wgrad stages exceed the shared memory of a CTA");
+  static_assert((4 * kWStages + 4) * 8 + 4 <= 256, "grouped wgrad barriers exceed their area");
 };
+
+// Rows of a group's block kb that belong to it, and whether its last MMA step is cut.
+__device__ __forceinline__ int valid_rows(int size, int kb) { return min(kBK, size - kb * kBK); }
+__device__ __forceinline__ bool is_cut(int valid) { return (valid & 15) != 0; }
 
 template <bool ACC>
 __global__ void __launch_bounds__(kWThreads, 1)
@@ -351,16 +364,20 @@ __global__ void __launch_bounds__(kWThreads, 1)
   uint8_t* staging = smem + kWStages * S::kStageBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * S::kOutBytes);
   uint64_t* empty = full + kWStages;
-  uint64_t* acc_full = empty + kWStages;
+  uint64_t* cut = empty + kWStages;
+  uint64_t* zeroed = cut + kWStages;
+  uint64_t* acc_full = zeroed + kWStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   Lists l;
   l.row = reinterpret_cast<int*>(staging + 8 * S::kOutBytes + 256);
   l.tile = l.row + kMaxGroups + 2;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0);  // uniform for the compiler too
   const int lane = threadIdx.x & 31;
-  const int tiles_m = (g.n + 127) / 128, tiles_n = (g.k + 255) / 256;
+  const uint32_t cta = cluster_ctarank();  // 0: leader, 1: peer
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles_m = (g.n + 255) / 256, tiles_n = (g.k + 255) / 256;
   const int per_group = tiles_m * tiles_n;
   const int tiles = g.groups * per_group;
 
@@ -368,20 +385,22 @@ __global__ void __launch_bounds__(kWThreads, 1)
     for (int s = 0; s < kWStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&cut[s], 1);
+      mbar_init(&zeroed[s], 2);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);
+      mbar_init(&acc_empty[a], 16);
     }
     fence_barrier_init();
     tma_prefetch(&tma_dy);
     tma_prefetch(&tma_x);
     tma_prefetch(&tma_c);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, S::kTmemCols);
-  build_lists(l, g, kWK, 1);  // "tiles": the group's row blocks
+  if (warp == 1) tmem_alloc_pair(tmem_slot, S::kTmemCols);
+  build_lists(l, g, kBK, 1);  // "tiles": the group's row blocks
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();  // both CTAs' barriers initialised and TMEM allocated before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -390,83 +409,125 @@ __global__ void __launch_bounds__(kWThreads, 1)
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = pair; t < tiles && ok; t += pairs) {
         const int e = t / per_group;
         int tm, tn;
         tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
-        const int blocks = l.tile[e + 1] - l.tile[e];
-        const int m0 = tm * 128, n0 = tn * 256;
+        const int size = l.row[e + 1] - l.row[e], blocks = l.tile[e + 1] - l.tile[e];
+        const int m0 = tm * 256 + int(cta) * 128, n0 = tn * 256 + int(cta) * 128;
         for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) { ok = false; break; }
           uint8_t* sa = smem + s * S::kStageBytes;
           uint8_t* sb = sa + S::kABytes;
-          mbar_expect_tx(&full[s], S::kStageBytes);
-          const int r0 = l.row[e] + kb * kWK;
-          #pragma unroll
-          for (int c = 0; c < 2; ++c) tma_load_2d(sa + c * S::kChunkBytes, &tma_dy, &full[s], m0 + 64 * c, r0, g.err);
-          #pragma unroll
-          for (int c = 0; c < 4; ++c) tma_load_2d(sb + c * S::kChunkBytes, &tma_x, &full[s], n0 + 64 * c, r0, g.err);
+          uint32_t bar;
+          if (is_cut(valid_rows(size, kb))) {
+            if (cta == 0) mbar_arrive(&full[s]);
+            mbar_expect_tx(&cut[s], S::kStageBytes);
+            bar = mapa_shared(&cut[s], cta);
+          } else {
+            if (cta == 0) mbar_expect_tx(&full[s], 2 * S::kStageBytes);  // both CTAs' halves
+            bar = mapa_shared(&full[s], 0);
+          }
+          const int r0 = l.row[e] + kb * kBK;
+          tma_load_2d_pair(sa, &tma_dy, bar, m0, r0, g.err);
+          tma_load_2d_pair(sa + S::kChunkBytes, &tma_dy, bar, m0 + 64, r0, g.err);
+          tma_load_2d_pair(sb, &tma_x, bar, n0, r0, g.err);
+          tma_load_2d_pair(sb + S::kChunkBytes, &tma_x, bar, n0 + 64, r0, g.err);
           if (++s == kWStages) { s = 0; ph ^= 1; }
         }
       }
+      // Producer tail: every stage released, so no commit can arrive after this CTA exits.
+      for (int j = 0; j < kWStages && ok; ++j) {
+        if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) break;
+        if (++s == kWStages) { s = 0; ph ^= 1; }
+      }
     }
   } else if (warp == 1) {
-    // the whole warp walks the stages (it zeroes a cut block together); lane 0 issues
-    constexpr uint32_t idesc = idesc_bf16_f32(128, 256, 1, 1);
-    int s = 0, i = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int e = t / per_group;
-      const int size = l.row[e + 1] - l.row[e];
-      const int blocks = l.tile[e + 1] - l.tile[e];
-      for (int kb = 0; kb < blocks; ++kb) {
-        const int a = i & 1;
-        const uint32_t d = tmem_base + a * 256;
-        if (kb % kWChunk == 0) {
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait))) { ok = false; break; }
-          tc_fence_after();
-        }
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[s], ph, g.err, kErrMmaWait))) { ok = false; break; }
-        const int valid = min(kWK, size - kb * kWK);
-        const int steps = (valid + 15) / 16;
-        uint8_t* stage = smem + s * S::kStageBytes;
-        if (valid < 16 * steps) {
-          // MN-major chunks are rows of 128 bytes: rows valid .. 16 * steps hold the next
-          // group's rows (zeroed in both operands: 0 * inf would not be 0)
-          const int bytes = (16 * steps - valid) * 128;
-          #pragma unroll 1
-          for (int c = 0; c < 6; ++c)
-            for (int b = lane * 16; b < bytes; b += 512)
-              *reinterpret_cast<uint4*>(stage + c * S::kChunkBytes + valid * 128 + b) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async();
-          __syncwarp();
-        }
-        if (lane == 0) {
-          tc_fence_after();
-          const uint32_t sa = smem_u32(stage);
-          const uint32_t sb = sa + S::kABytes;
-          for (int kk = 0; kk < steps; ++kk)
-            umma_bf16(d, smem_desc_sw128(sa + kk * 2048, S::kChunkBytes, 1024),
-                      smem_desc_sw128(sb + kk * 2048, S::kChunkBytes, 1024), idesc, kb % kWChunk != 0 || kk != 0);
-          umma_commit(&empty[s]);
-        }
-        __syncwarp();
-        if (++s == kWStages) { s = 0; ph ^= 1; }
-        if (kb % kWChunk == kWChunk - 1 || kb == blocks - 1) {
-          if (lane == 0) umma_commit(&acc_full[a]);
-          __syncwarp();
+    if (cta == 0) {  // the whole warp walks, one lane issues
+      const uint32_t issue = elect_one();
+      constexpr uint32_t idesc = idesc_bf16_f32(256, 256, 1, 1);
+      const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(empty), bar1 = mapa_shared(empty, 1);
+      const uint32_t done0 = smem_u32(acc_full), done1 = mapa_shared(acc_full, 1);
+      int s = 0, i = 0;
+      uint32_t ph = 0, zph = 0;  // zph: a parity bit per stage
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const int e = t / per_group;
+        int left = __shfl_sync(0xFFFFFFFFu, l.row[e + 1] - l.row[e], 0);  // rows still to add
+        while (left > 0 && ok) {  // one accumulator
+          const int a = i & 1;
+          const uint32_t d = tmem_base + a * 256;
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster(&acc_empty[a], ((i >> 1) & 1) ^ 1, g.err, kErrMmaWait)) ||
+              !tmem_span_ok(d, tmem_base, S::kTmemCols, 256, g.err)) {
+            ok = false;
+            break;
+          }
+          uint32_t onto = 0;
+          for (int kb = 0; kb < kWChunk && left > 0; ++kb) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[s], ph, g.err, kErrMmaWait))) { ok = false; break; }
+            const uint32_t sa = sbase + s * S::kStageBytes;
+            const uint64_t da = smem_desc_sw128(sa, S::kChunkBytes, 1024);
+            const uint64_t db = smem_desc_sw128(sa + S::kABytes, S::kChunkBytes, 1024);
+            if (left >= kBK) {
+              tc_fence_after();
+              #pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk)
+                umma_bf16_pair_if(issue, d, da + kk * (2048 / 16), db + kk * (2048 / 16), idesc, kk == 0 ? onto : 1u);
+            } else {
+              if (is_cut(left)) {
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster(&zeroed[s], (zph >> s) & 1, g.err, kErrMmaWait))) { ok = false; break; }
+                zph ^= 1u << s;
+              }
+              tc_fence_after();
+              for (int kk = 0; kk * 16 < left; ++kk)
+                umma_bf16_pair_if(issue, d, da + kk * (2048 / 16), db + kk * (2048 / 16), idesc, kk == 0 ? onto : 1u);
+            }
+            umma_commit_pair_if(issue, bar0 + s * 8);
+            umma_commit_pair_if(issue, bar1 + s * 8);
+            if (++s == kWStages) { s = 0; ph ^= 1; }
+            onto = 1;
+            left -= kBK;
+          }
+          if (!ok) break;
+          umma_commit_pair_if(issue, done0 + a * 8);
+          umma_commit_pair_if(issue, done1 + a * 8);
           ++i;
         }
       }
     }
+  } else if (warp == 2) {
+    int s = 0;  // stage of the next block
+    uint32_t cph = 0;
+    for (int t = pair; t < tiles; t += pairs) {
+      const int e = t / per_group;
+      const int size = l.row[e + 1] - l.row[e], blocks = l.tile[e + 1] - l.tile[e];
+      if (blocks == 0) continue;
+      const int last = (s + blocks - 1) % kWStages;
+      s = (s + blocks) % kWStages;
+      const int valid = valid_rows(size, blocks - 1);
+      if (!is_cut(valid)) continue;
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&cut[last], (cph >> last) & 1, g.err, kErrMmaWait))) break;
+      cph ^= 1u << last;
+      // MN-major chunks are rows of 128 bytes; both operands are zeroed (0 * inf is not 0)
+      const int bytes = (((valid + 15) & ~15) - valid) * 128;
+      uint8_t* stage = smem + last * S::kStageBytes + valid * 128;
+      #pragma unroll 1
+      for (int c = 0; c < 4; ++c)
+        for (int b = lane * 16; b < bytes; b += 512)
+          *reinterpret_cast<uint4*>(stage + c * S::kChunkBytes + b) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(mapa_shared(&zeroed[last], 0));
+    }
   } else {
     const int q = warp & 3;           // TMEM lane quarter this warp may access
-    const int half = (warp - 2) >> 2;  // columns 128 * half .. + 127 of the tile
-    uint8_t* buf = staging + (warp - 2) * S::kOutBytes;
+    const int half = (warp - 3) >> 2;  // columns 128 * half .. + 127 of the tile
+    uint8_t* buf = staging + (warp - 3) * S::kOutBytes;
+    const uint32_t acc_empty_leader0 = mapa_shared(&acc_empty[0], 0);
+    const uint32_t acc_empty_leader1 = mapa_shared(&acc_empty[1], 0);
     int i = 0, turn = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = pair; t < tiles && ok; t += pairs) {
       const int e = t / per_group;
       const int blocks = l.tile[e + 1] - l.tile[e];
       if (blocks == 0 && ACC) continue;
@@ -487,12 +548,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[a]);
+        if (lane == 0) mbar_arrive_remote(a == 0 ? acc_empty_leader0 : acc_empty_leader1);
       }
       if (!ok) break;
       int tm, tn;
       tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
-      const int row0 = tm * 128 + q * 32, col0 = tn * 256 + half * 128;
+      const int row0 = tm * 256 + int(cta) * 128 + q * 32, col0 = tn * 256 + half * 128;
       if (row0 >= g.n) continue;
       #pragma unroll
       for (int j = 0; j < 8; ++j) {  // 16 columns at a time through one of two buffers
@@ -519,10 +580,10 @@ __global__ void __launch_bounds__(kWThreads, 1)
   }
 
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();  // no CTA leaves while its pair may still touch its barriers or TMEM
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, S::kTmemCols);
+    tmem_dealloc_pair(tmem_base, S::kTmemCols);
   }
 }
 
@@ -536,10 +597,11 @@ int num_sms() {
   return counts[dev];
 }
 
-// Pairs of CTAs that can be resident at once (a persistent grid larger than that only queues).
-template <int TN, bool W_MN>
-void launch_rows(int64_t tiles, const CUtensorMap& tw, const CUtensorMap& ta, const Args& g, cudaStream_t st) {
-  auto kernel = grouped_rows_kernel<TN, W_MN>;
+// ``kernel`` on min(tiles, the pairs that can be resident at once) CTA pairs: a persistent grid
+// larger than that would only queue. ``resident``: that number by device, 0 before it is known.
+template <typename Kernel, typename... A>
+void launch_pairs(Kernel kernel, int (&resident)[64], int threads, int smem, int64_t tiles, cudaStream_t st,
+                  const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -548,16 +610,15 @@ void launch_rows(int64_t tiles, const CUtensorMap& tw, const CUtensorMap& ta, co
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel starts with pdl_enter()
   attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.blockDim = dim3(192, 1, 1);
-  cfg.dynamicSmemBytes = RowTile<TN>::kSmem;
+  cfg.blockDim = dim3(unsigned(threads), 1, 1);
+  cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  static int resident[64] = {0};
   int dev = 0;
   RESIHP_CUDA_CHECK(cudaGetDevice(&dev));
   if (resident[dev] == 0) {
-    RESIHP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowTile<TN>::kSmem));
+    RESIHP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cfg.gridDim = dim3(2, 1, 1);
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
@@ -568,7 +629,20 @@ void launch_rows(int64_t tiles, const CUtensorMap& tw, const CUtensorMap& ta, co
   }
   cfg.gridDim = dim3(2 * unsigned(std::min<int64_t>(tiles, resident[dev])), 1, 1);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  RESIHP_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, tw, ta, g));
+  RESIHP_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+template <int TN, bool W_MN>
+void launch_rows(int64_t tiles, const CUtensorMap& tw, const CUtensorMap& ta, const Args& g, cudaStream_t st) {
+  static int resident[64] = {0};
+  launch_pairs(grouped_rows_kernel<TN, W_MN>, resident, 192, RowTile<TN>::kSmem, tiles, st, tw, ta, g);
+}
+
+template <bool ACC>
+void launch_wgrad(int64_t tiles, const CUtensorMap& tdy, const CUtensorMap& tx, const CUtensorMap& tc, const Args& g,
+                  cudaStream_t st) {
+  static int resident[64] = {0};
+  launch_pairs(grouped_wgrad_kernel<ACC>, resident, kWThreads, WgradTile::kSmem, tiles, st, tdy, tx, tc, g);
 }
 
 template <int TN>
@@ -612,16 +686,14 @@ void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, flo
     if (!accumulate) RESIHP_CUDA_CHECK(cudaMemsetAsync(c, 0, sizeof(float) * size_t(s.groups) * s.n * s.k, st));
     return;
   }
-  const int64_t tiles = int64_t(s.groups) * ((s.n + 127) / 128) * ((s.k + 255) / 256);
+  const int64_t tiles = int64_t(s.groups) * ((s.n + 255) / 256) * ((s.k + 255) / 256);
   RESIHP_CHECK(tiles <= INT32_MAX, "grouped products: too many tiles");
-  const CUtensorMap ta = make_tma_2d_bf16(dy, s.rows, s.n, lddy, 64, kWK);
-  const CUtensorMap tb = make_tma_2d_bf16(x, s.rows, s.k, ldx, 64, kWK);
+  const CUtensorMap tdy = make_tma_2d_bf16(dy, s.rows, s.n, lddy, 64, kBK);
+  const CUtensorMap tx = make_tma_2d_bf16(x, s.rows, s.k, ldx, 64, kBK);
   const CUtensorMap tc = make_tma_3d_f32(c, s.groups, s.n, s.k, 32);
   const Args g{c, 0, s.offsets, s.groups, s.rows, s.n, s.k, err};
-  auto kernel = accumulate ? grouped_wgrad_kernel<true> : grouped_wgrad_kernel<false>;
-  RESIHP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WgradTile::kSmem));
-  const int grid = int(std::min<int64_t>(tiles, num_sms()));
-  RESIHP_CUDA_CHECK(launch_pdl(kernel, grid, kWThreads, WgradTile::kSmem, st, ta, tb, tc, g));
+  if (accumulate) launch_wgrad<true>(tiles, tdy, tx, tc, g, st);
+  else launch_wgrad<false>(tiles, tdy, tx, tc, g, st);
 }
 
 }  // namespace resihp
