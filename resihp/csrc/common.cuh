@@ -351,8 +351,14 @@ __device__ __forceinline__ void tma_add_3d_f32(const CUtensorMap* map, const voi
                : "memory");
 }
 
-// At most one committed bulk group of this thread is still reading its shared memory.
-__device__ __forceinline__ void bulk_wait_read_keep1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+// Start bringing a tile of an fp32 3-D map into L2; nothing waits for it.
+__device__ __forceinline__ void tma_prefetch_3d_f32(const CUtensorMap* map, int x, int y, int z, int* err = nullptr) {
+  if (!bounds_ok((x & 3) == 0 && x >= 0 && y >= 0 && z >= 0, err)) return;
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
@@ -489,6 +495,45 @@ __device__ __forceinline__ void umma_commit_pair_if(uint32_t issue, uint32_t bar
       "setp.ne.b32 q, %1, 0;\n\t"
       "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar_cluster),
       "r"(issue)
+      : "memory");
+}
+
+// Loads and expectations of a producer warp in the same manner (see tma_load_2d_pair).
+__device__ __forceinline__ void tma_load_2d_pair_if(uint32_t issue, uint32_t dst, const CUtensorMap* map,
+                                                    uint32_t bar_cluster, int x, int y, int* err = nullptr) {
+  if (!bounds_ok((x & 7) == 0 && x >= 0 && y >= 0 && (dst & 1023u) == 0, err)) return;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair_if(uint32_t issue, uint32_t dst, const CUtensorMap* map,
+                                                    uint32_t bar_cluster, int x, int y, int z, int* err = nullptr) {
+  if (!bounds_ok((x & 7) == 0 && x >= 0 && y >= 0 && z >= 0 && (dst & 1023u) == 0, err)) return;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_if(uint32_t issue, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_if(uint32_t issue, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"(issue)
       : "memory");
 }
 

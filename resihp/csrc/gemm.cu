@@ -504,16 +504,17 @@ static CUtensorMap make_tma_3d(CUtensorMapDataType type, int size, CUtensorMapSw
 }
 
 // ``planes`` row-major [rows, cols] matrices ``plane_ld`` elements apart, tiled by (box_cols,
-// box_rows, 1): a box never reaches into the next plane. bf16 with 128-byte swizzle (loads
-// read zeros past the edges), fp32 with 64-byte swizzle (box_cols = 16; stores are clipped).
+// box_rows, 1): a box never reaches past a matrix's edge. bf16 with 128-byte swizzle
+// (loads read zeros past the edges), fp32 with 128-byte swizzle (box_cols = 32; stores are
+// clipped).
 CUtensorMap make_tma_3d_bf16(const void* base, int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld,
                              int box_cols, int box_rows) {
   return make_tma_3d(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, base, planes, rows, cols, ld,
                      plane_ld, box_cols, box_rows);
 }
 CUtensorMap make_tma_3d_f32(const void* base, int64_t planes, int64_t rows, int64_t cols, int box_rows) {
-  return make_tma_3d(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, CU_TENSOR_MAP_SWIZZLE_64B, base, planes, rows, cols, cols,
-                     rows * cols, 16, box_rows);
+  return make_tma_3d(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, CU_TENSOR_MAP_SWIZZLE_128B, base, planes, rows, cols, cols,
+                     rows * cols, 32, box_rows);
 }
 
 static int num_sms() {

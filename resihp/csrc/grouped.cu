@@ -119,7 +119,7 @@ struct RowTile {
   static constexpr int kWBytes = 128 * kBK * 2;         // this CTA's 128 features
   static constexpr int kABytes = TN / 2 * kBK * 2;      // this CTA's half of the rows
   static constexpr int kStageBytes = kWBytes + kABytes;
-  static constexpr int kStages = TN == 256 ? 6 : 10;
+  static constexpr int kStages = TN == 256 ? 6 : 8;
   static constexpr int kListBytes = 2 * (kMaxGroups + 2) * 4;
   static constexpr int kSmem = kStages * kStageBytes + 1024 /*align*/ + 256 /*barriers*/ + kListBytes;
   static constexpr int kTmemCols = 2 * TN;
@@ -192,38 +192,39 @@ __global__ void __launch_bounds__(192, 1)
   const int tiles = l.tile[g.groups + 1];   // and those of the rows behind the last group
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0, e = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int t = pair; t < work && ok; t += pairs) {
-        e = group_of(l, g.groups, t, e);
-        const RowSpan p = span_of<TN>(l, e, t, tiles_f);
-        // each CTA brings its features and its half of the MMA's N rows
-        const int f0 = p.f0 + int(cta) * 128, r0 = p.row0 + int(cta) * (mma_rows(p.rows) >> 1);
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) { ok = false; break; }
-          uint8_t* sw = smem + s * S::kStageBytes;
-          uint8_t* sa = sw + S::kWBytes;
-          if (cta == 0) mbar_expect_tx(&full[s], 2 * S::kStageBytes);  // both CTAs' parts
-          const uint32_t bar = mapa_shared(&full[s], 0);
-          const int k0 = kb * kBK;
-          if (W_MN) {
-            tma_load_3d_pair(sw, &tma_w, bar, f0, k0, e, g.err);
-            tma_load_3d_pair(sw + 8192, &tma_w, bar, f0 + 64, k0, e, g.err);
-          } else {
-            tma_load_3d_pair(sw, &tma_w, bar, k0, f0, e, g.err);
-          }
-          tma_load_2d_pair(sa, &tma_a, bar, k0, r0, g.err);
-          if (++s == kStages) { s = 0; ph ^= 1; }
+    // the whole warp walks, one lane issues
+    const uint32_t issue = elect_one(), lead = cta == 0 ? issue : 0u;
+    const uint32_t sbase = smem_u32(smem), fbase = smem_u32(full), fleader = mapa_shared(full, 0);
+    int s = 0, e = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = pair; t < work && ok; t += pairs) {
+      e = group_of(l, g.groups, t, e);
+      const RowSpan p = span_of<TN>(l, e, t, tiles_f);
+      // each CTA brings its features and its half of the MMA's N rows
+      const int f0 = p.f0 + int(cta) * 128;
+      const int r0 = __shfl_sync(0xFFFFFFFFu, p.row0 + int(cta) * (mma_rows(p.rows) >> 1), 0);
+      const int plane = __shfl_sync(0xFFFFFFFFu, e, 0);
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait))) { ok = false; break; }
+        const uint32_t sw = sbase + s * S::kStageBytes, bar = fleader + s * 8;
+        mbar_expect_tx_if(lead, fbase + s * 8, 2 * S::kStageBytes);  // both CTAs' parts
+        const int k0 = kb * kBK;
+        if (W_MN) {
+          tma_load_3d_pair_if(issue, sw, &tma_w, bar, f0, k0, plane, g.err);
+          tma_load_3d_pair_if(issue, sw + 8192, &tma_w, bar, f0 + 64, k0, plane, g.err);
+        } else {
+          tma_load_3d_pair_if(issue, sw, &tma_w, bar, k0, f0, plane, g.err);
         }
-      }
-      // Producer tail: wait until the leader has released every stage, so no pair-MMA
-      // commit can arrive on this CTA's barriers after it exits.
-      for (int j = 0; j < kStages && ok; ++j) {
-        if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) break;
+        tma_load_2d_pair_if(issue, sw + S::kWBytes, &tma_a, bar, k0, r0, g.err);
         if (++s == kStages) { s = 0; ph ^= 1; }
       }
+    }
+    // Producer tail: wait until the leader has released every stage, so no pair-MMA commit can
+    // arrive on this CTA's barriers after it exits.
+    for (int j = 0; j < kStages && ok; ++j) {
+      if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) break;
+      if (++s == kStages) { s = 0; ph ^= 1; }
     }
   } else if (warp == 1) {
     if (cta == 0) {  // the whole warp walks, one lane issues
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(192, 1)
 // MMAs go on in the other accumulator: 4.8e-7 at every length, for 3 % of the rate (1222
 // against 1255 TF/s, two groups of 8192 rows; every 256 rows 2.7e-7 at 1125). Eight epilogue
 // warps per CTA keep 128 columns of a row per thread. The finished tile leaves through shared
-// memory as bulk stores or bulk additions (whole 64-byte runs, clipped at the matrix's edges
+// memory as bulk stores or bulk additions (whole 128-byte runs, clipped at the matrix's edges
 // by the map): each element is added to once per launch, so no order can change the sum.
 //
 // A group's last block holds rows of the next group where its length is no multiple of 64.
@@ -340,7 +341,7 @@ struct WgradTile {
   static constexpr int kChunkBytes = 64 * kBK * 2;  // 64 columns of a block, MN-major
   static constexpr int kABytes = 2 * kChunkBytes;   // this CTA's 128 columns of dy, then of x
   static constexpr int kStageBytes = 4 * kChunkBytes;
-  static constexpr int kOutBytes = 2 * 32 * 16 * 4;  // per epilogue warp: two 32 x 16 fp32 buffers
+  static constexpr int kOutBytes = 32 * 32 * 4;  // per epilogue warp: 32 x 32 fp32
   static constexpr int kListBytes = 2 * (kMaxGroups + 2) * 4;
   static constexpr int kSmem = kWStages * kStageBytes + 8 * kOutBytes + 1024 + 256 + kListBytes;
   static constexpr int kTmemCols = 512;
@@ -405,42 +406,42 @@ __global__ void __launch_bounds__(kWThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        const int e = t / per_group;
-        int tm, tn;
-        tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
-        const int size = l.row[e + 1] - l.row[e], blocks = l.tile[e + 1] - l.tile[e];
-        const int m0 = tm * 256 + int(cta) * 128, n0 = tn * 256 + int(cta) * 128;
-        for (int kb = 0; kb < blocks; ++kb) {
-          if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) { ok = false; break; }
-          uint8_t* sa = smem + s * S::kStageBytes;
-          uint8_t* sb = sa + S::kABytes;
-          uint32_t bar;
-          if (is_cut(valid_rows(size, kb))) {
-            if (cta == 0) mbar_arrive(&full[s]);
-            mbar_expect_tx(&cut[s], S::kStageBytes);
-            bar = mapa_shared(&cut[s], cta);
-          } else {
-            if (cta == 0) mbar_expect_tx(&full[s], 2 * S::kStageBytes);  // both CTAs' halves
-            bar = mapa_shared(&full[s], 0);
-          }
-          const int r0 = l.row[e] + kb * kBK;
-          tma_load_2d_pair(sa, &tma_dy, bar, m0, r0, g.err);
-          tma_load_2d_pair(sa + S::kChunkBytes, &tma_dy, bar, m0 + 64, r0, g.err);
-          tma_load_2d_pair(sb, &tma_x, bar, n0, r0, g.err);
-          tma_load_2d_pair(sb + S::kChunkBytes, &tma_x, bar, n0 + 64, r0, g.err);
-          if (++s == kWStages) { s = 0; ph ^= 1; }
+    // the whole warp walks, one lane issues
+    const uint32_t issue = elect_one(), lead = cta == 0 ? issue : 0u;
+    const uint32_t sbase = smem_u32(smem), fbase = smem_u32(full), fleader = mapa_shared(full, 0);
+    const uint32_t cbase = smem_u32(cut), cown = mapa_shared(cut, cta);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      const int e = t / per_group;
+      int tm, tn;
+      tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
+      int r0 = __shfl_sync(0xFFFFFFFFu, l.row[e], 0);
+      int left = __shfl_sync(0xFFFFFFFFu, l.row[e + 1], 0) - r0;
+      const int m0 = tm * 256 + int(cta) * 128, n0 = tn * 256 + int(cta) * 128;
+      for (; left > 0; left -= kBK, r0 += kBK) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait))) { ok = false; break; }
+        uint32_t bar = fleader + s * 8;
+        if (left < kBK && is_cut(left)) {
+          mbar_arrive_if(lead, fbase + s * 8);
+          mbar_expect_tx_if(issue, cbase + s * 8, S::kStageBytes);
+          bar = cown + s * 8;
+        } else {
+          mbar_expect_tx_if(lead, fbase + s * 8, 2 * S::kStageBytes);  // both CTAs' halves
         }
-      }
-      // Producer tail: every stage released, so no commit can arrive after this CTA exits.
-      for (int j = 0; j < kWStages && ok; ++j) {
-        if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) break;
+        const uint32_t sa = sbase + s * S::kStageBytes;
+        tma_load_2d_pair_if(issue, sa, &tma_dy, bar, m0, r0, g.err);
+        tma_load_2d_pair_if(issue, sa + S::kChunkBytes, &tma_dy, bar, m0 + 64, r0, g.err);
+        tma_load_2d_pair_if(issue, sa + 2 * S::kChunkBytes, &tma_x, bar, n0, r0, g.err);
+        tma_load_2d_pair_if(issue, sa + 3 * S::kChunkBytes, &tma_x, bar, n0 + 64, r0, g.err);
         if (++s == kWStages) { s = 0; ph ^= 1; }
       }
+    }
+    // Producer tail: every stage released, so no commit can arrive after this CTA exits.
+    for (int j = 0; j < kWStages && ok; ++j) {
+      if (!mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait)) break;
+      if (++s == kWStages) { s = 0; ph ^= 1; }
     }
   } else if (warp == 1) {
     if (cta == 0) {  // the whole warp walks, one lane issues
@@ -525,17 +526,32 @@ __global__ void __launch_bounds__(kWThreads, 1)
     uint8_t* buf = staging + (warp - 3) * S::kOutBytes;
     const uint32_t acc_empty_leader0 = mapa_shared(&acc_empty[0], 0);
     const uint32_t acc_empty_leader1 = mapa_shared(&acc_empty[1], 0);
-    int i = 0, turn = 0;
+    int i = 0;
     bool ok = true;
+    // This warp's part of tile t, brought into L2 ahead of the additions to it: a tile of one
+    // accumulator during the tile before it, a longer one during its last accumulator.
+    auto prefetch = [&](int t, bool ahead) {
+      if (t >= tiles) return;
+      const int e = t / per_group;
+      const int blocks = l.tile[e + 1] - l.tile[e];
+      if (blocks == 0 || ahead != (blocks <= kWChunk)) return;
+      int tm, tn;
+      tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
+      const int row0 = tm * 256 + int(cta) * 128 + q * 32, col0 = tn * 256 + half * 128 + lane * 32;
+      if (lane < 4 && row0 < g.n && col0 < g.k) tma_prefetch_3d_f32(&tma_c, col0, row0, e, g.err);
+    };
+    if (ACC) prefetch(pair, true);
     for (int t = pair; t < tiles && ok; t += pairs) {
       const int e = t / per_group;
       const int blocks = l.tile[e + 1] - l.tile[e];
+      if (ACC) prefetch(t + pairs, true);
       if (blocks == 0 && ACC) continue;
       float acc[128];
       #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
       for (int c = 0; c < blocks; c += kWChunk, ++i) {
         const int a = i & 1;
+        if (ACC && c + kWChunk >= blocks) prefetch(t, false);
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[a], (i >> 1) & 1, g.err, kErrEpiWait))) { ok = false; break; }
         tc_fence_after();
         #pragma unroll
@@ -556,23 +572,21 @@ __global__ void __launch_bounds__(kWThreads, 1)
       const int row0 = tm * 256 + int(cta) * 128 + q * 32, col0 = tn * 256 + half * 128;
       if (row0 >= g.n) continue;
       #pragma unroll
-      for (int j = 0; j < 8; ++j) {  // 16 columns at a time through one of two buffers
-        if (col0 + j * 16 < g.k) {
-          if (lane == 0) bulk_wait_read_keep1();
+      for (int j = 0; j < 4; ++j) {  // 32 columns at a time
+        if (col0 + j * 32 < g.k) {
+          if (lane == 0) bulk_wait_read_all();
           __syncwarp();
-          uint8_t* b = buf + turn * (S::kOutBytes / 2);
           #pragma unroll
-          for (int x = 0; x < 4; ++x)  // the map's 64-byte swizzle: 16-byte unit x of row r is at x ^ (r / 2) % 4
-            *reinterpret_cast<float4*>(b + lane * 64 + ((x ^ ((lane >> 1) & 3)) << 4)) =
-                make_float4(acc[j * 16 + 4 * x], acc[j * 16 + 4 * x + 1], acc[j * 16 + 4 * x + 2], acc[j * 16 + 4 * x + 3]);
+          for (int x = 0; x < 8; ++x)  // the map's 128-byte swizzle: 16-byte unit x of row r is at x ^ r % 8
+            *reinterpret_cast<float4*>(buf + lane * 128 + ((x ^ (lane & 7)) << 4)) =
+                make_float4(acc[j * 32 + 4 * x], acc[j * 32 + 4 * x + 1], acc[j * 32 + 4 * x + 2], acc[j * 32 + 4 * x + 3]);
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            if (ACC) tma_add_3d_f32(&tma_c, b, col0 + j * 16, row0, e, g.err);
-            else tma_store_3d_f32(&tma_c, b, col0 + j * 16, row0, e, g.err);
+            if (ACC) tma_add_3d_f32(&tma_c, buf, col0 + j * 32, row0, e, g.err);
+            else tma_store_3d_f32(&tma_c, buf, col0 + j * 32, row0, e, g.err);
             bulk_commit();
           }
-          turn ^= 1;
         }
       }
     }
@@ -673,8 +687,11 @@ void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_
   if (s.rows == 0) return;
   RESIHP_CHECK(reinterpret_cast<uintptr_t>(c) % 16 == 0 && ldc % 8 == 0, "grouped output must be 16-byte aligned");
   const Args g{c, ldc, s.offsets, s.groups, s.rows, s.n, s.k, err};
-  // Few rows per group: narrow row tiles, whose smaller stages keep ten weight tiles in flight.
-  if (s.rows <= int64_t(48) * s.groups) launch_rows_tn<64>(a, lda, w, ldw, w_group, w_mn, s, g, st);
+  // Few rows per group: the weights' bytes set the time, and narrow row tiles leave room for
+  // eight of their stages in flight instead of six. At 100 rows a group (eight groups, 2048 >
+  // 11008) 64.3 against 66.7 us, at 94 uneven ones (64 groups, 1024 > 1416) 44.3 against 46.9;
+  // at 150 uneven ones 73.7 against 70.6: groups of more than 128 rows read their weights twice.
+  if (s.rows <= int64_t(112) * s.groups) launch_rows_tn<128>(a, lda, w, ldw, w_group, w_mn, s, g, st);
   else launch_rows_tn<256>(a, lda, w, ldw, w_group, w_mn, s, g, st);
 }
 
