@@ -7,6 +7,10 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <atomic>
 #include <mutex>
 #include <csignal>
 #include <execinfo.h>
@@ -461,6 +465,158 @@ void grouped_wgrad_t(torch::Tensor dy, torch::Tensor x, torch::Tensor offsets, t
                 error_word(dy.device()), cur_stream());
 }
 
+// ---- differentiable forms -------------------------------------------------------------------
+// The autograd nodes of the operators above. They are C++ so that a backward pass neither
+// enters the interpreter nor waits for its lock: at the sizes where such an operator's kernels
+// take 5 to 20 us, Python nodes made forward and backward of one of them 75 to 105 us of host
+// time.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<torch::Tensor>;
+
+// Kernels launched by backward passes (the launch counter adds them to what Python calls).
+static std::atomic<int64_t> g_backward_launches{0};
+static void count_backward(int64_t n) { g_backward_launches.fetch_add(n, std::memory_order_relaxed); }
+
+// These gradients have no derivative of their own: asking for one raises.
+static variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice an operator of resihp whose gradient has no derivative", int64_t(grads.size()));
+  return (*error)(std::move(grads));
+}
+
+static OptTensor rows_of(const OptTensor& t) { return t.has_value() ? OptTensor(t->contiguous()) : c10::nullopt; }
+
+struct DropoutNode : torch::autograd::Function<DropoutNode> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, int64_t drop, int64_t seed, int64_t offset,
+                               int64_t first, const OptTensor& state, const OptTensor& residual) {
+    ctx->saved_data["args"] = std::vector<int64_t>{drop, seed, offset, first, residual.has_value(), state.has_value()};
+    if (state.has_value()) ctx->save_for_backward({*state});
+    return dropout_t(x.contiguous(), rows_of(residual), drop, seed, offset, state, first);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto a = ctx->saved_data["args"].toIntVector();
+    OptTensor state;
+    if (a[5]) state = ctx->get_saved_variables()[0];
+    torch::Tensor dx;
+    if (ctx->needs_input_grad(0)) {
+      dx = dropout_t(grads[0].contiguous(), c10::nullopt, a[0], a[1], a[2], state, a[3]);
+      count_backward(1);
+    }
+    return once({dx, {}, {}, {}, {}, {}, a[4] ? grads[0] : torch::Tensor()});
+  }
+};
+
+struct RouteNode : torch::autograd::Function<RouteNode> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, int64_t k, bool normalize) {
+    const auto rows = logits.stride(1) == 1 ? logits : logits.contiguous();
+    auto out = moe_route_t(rows, k, normalize);
+    ctx->mark_non_differentiable({out[1], out[2], out[3]});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({rows, out[0], out[1]});
+    ctx->saved_data["normalize"] = normalize;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {{}, {}, {}};
+    const auto saved = ctx->get_saved_variables();
+    count_backward(1);
+    return once({moe_route_bwd_t(saved[0], saved[1], saved[2], grads[0].contiguous(),
+                                 ctx->saved_data["normalize"].toBool()), {}, {}});
+  }
+};
+
+struct DispatchNode : torch::autograd::Function<DispatchNode> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& offsets,
+                               const torch::Tensor& slots) {
+    ctx->save_for_backward({offsets, slots});
+    return moe_scatter_t(x.contiguous(), offsets, slots);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    count_backward(1);
+    return once({moe_gather_t(grads[0].contiguous(), c10::nullopt, saved[0], saved[1], c10::nullopt), {}, {}});
+  }
+};
+
+struct CombineNode : torch::autograd::Function<CombineNode> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& y, const torch::Tensor& weights,
+                               const torch::Tensor& offsets, const torch::Tensor& slots, const OptTensor& residual) {
+    const auto rows = y.contiguous();
+    const auto w = weights.contiguous();
+    ctx->save_for_backward({rows, w, offsets, slots});
+    ctx->saved_data["residual"] = residual.has_value();
+    return moe_gather_t(rows, w, offsets, slots, rows_of(residual));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    std::vector<torch::Tensor> d(2);
+    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
+      d = moe_combine_bwd_t(grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3]);
+      count_backward(1);
+    }
+    return once({d[0], d[1], {}, {}, ctx->saved_data["residual"].toBool() ? grads[0] : torch::Tensor()});
+  }
+};
+
+// A tensor as TMA reads it: unit inner stride, 16-byte aligned base and outer strides (which no
+// two rows may share); anything else is copied.
+static torch::Tensor tiles_of(const torch::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && t.stride(d) > 0 && t.stride(d) % 8 == 0;
+  return ok ? t : torch::empty(t.sizes(), t.options()).copy_(t);
+}
+
+struct GroupedNode : torch::autograd::Function<GroupedNode> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& w,
+                               const torch::Tensor& offsets, const OptTensor& main_grad) {
+    const auto xt = tiles_of(x), wt = tiles_of(w);
+    ctx->save_for_backward({xt, wt, offsets});
+    if (main_grad.has_value()) ctx->saved_data["main_grad"] = *main_grad;
+    return grouped_rows_t(xt, wt, false, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto dy = tiles_of(grads[0]);
+    torch::Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) {
+      dx = grouped_rows_t(dy, saved[1], true, saved[2]);
+      count_backward(1);
+    }
+    const auto acc = ctx->saved_data.find("main_grad");
+    if (acc != ctx->saved_data.end()) {
+      grouped_wgrad_t(dy, saved[0], saved[2], acc->second.toTensor(), true);
+      count_backward(1);
+    } else if (ctx->needs_input_grad(1)) {
+      auto sum = torch::empty(saved[1].sizes(), saved[1].options().dtype(torch::kFloat));
+      grouped_wgrad_t(dy, saved[0], saved[2], sum, false);
+      count_backward(1);
+      dw = sum.to(saved[1].scalar_type());
+    }
+    return once({dx, dw, {}, {}});
+  }
+};
+
+static torch::Tensor dropout_ad(torch::Tensor x, int64_t drop, int64_t seed, int64_t offset, int64_t first,
+                                OptTensor state, OptTensor residual) {
+  return DropoutNode::apply(x, drop, seed, offset, first, state, residual);
+}
+static variable_list moe_route_ad(torch::Tensor logits, int64_t k, bool normalize) {
+  return RouteNode::apply(logits, k, normalize);
+}
+static torch::Tensor moe_dispatch_ad(torch::Tensor x, torch::Tensor offsets, torch::Tensor slots) {
+  return DispatchNode::apply(x, offsets, slots);
+}
+static torch::Tensor moe_combine_ad(torch::Tensor y, torch::Tensor weights, torch::Tensor offsets, torch::Tensor slots,
+                                    OptTensor residual) {
+  return CombineNode::apply(y, weights, offsets, slots, residual);
+}
+static torch::Tensor grouped_linear_ad(torch::Tensor x, torch::Tensor w, torch::Tensor offsets, OptTensor main_grad) {
+  return GroupedNode::apply(x, w, offsets, main_grad);
+}
+
 // ---- debugging aid: native backtrace on SIGSEGV ---------------------------------------
 
 static void crash_handler(int sig) {
@@ -700,6 +856,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_combine_bwd", &resihp::moe_combine_bwd_t);
   m.def("grouped_rows", &resihp::grouped_rows_t);
   m.def("grouped_wgrad", &resihp::grouped_wgrad_t);
+  m.def("backward_launches", [] { return resihp::g_backward_launches.load(); },
+        "kernels launched so far by the backward passes of the differentiable forms below");
+  m.def("dropout_ad", &resihp::dropout_ad);
+  m.def("moe_route_ad", &resihp::moe_route_ad);
+  m.def("moe_dispatch_ad", &resihp::moe_dispatch_ad);
+  m.def("moe_combine_ad", &resihp::moe_combine_ad);
+  m.def("grouped_linear_ad", &resihp::grouped_linear_ad);
   m.def("install_crash_handler", &resihp::install_crash_handler);
   m.def("symm_alloc", &resihp::symm_alloc_t);
   m.def("symm_open", &resihp::symm_open_t);

@@ -45,17 +45,42 @@ KERNELS_PER_CALL = {
     "adamw": 1, "embedding_fwd": 1, "embedding_bwd": 2, "xent_stats": 1, "xent_grad": 1,
     "dropout": 1, "moe_route": 2, "moe_route_bwd": 1, "moe_plan": 2, "moe_scatter": 1, "moe_gather": 1,
     "moe_combine_bwd": 1, "grouped_rows": 1, "grouped_wgrad": 1,
+    "dropout_ad": 1, "moe_route_ad": 2, "moe_dispatch_ad": 1, "moe_combine_ad": 1, "grouped_linear_ad": 1,
     "attn_fwd": 1, "attn_bwd": 3, "ag_gemm": 1, "gemm_rs": 1, "dp_allreduce_adamw": 1, "reshard_gather": 1,
 }
 
 
 class _Counting:
-    """Proxy over the extension module that counts kernel launches per entry point."""
+    """Proxy over the extension module that counts kernel launches per entry point.
+
+    The ``*_ad`` entry points launch their backward kernels from C++, where Python does not see
+    them: the module counts those itself.
+    """
 
     def __init__(self, module):
         self._module = module
-        self.launches = 0
-        self.enabled = False
+        self._called = 0
+        self._native = 0      # the module's count when counting began
+        self._enabled = False
+
+    @property
+    def enabled(self) -> bool:
+        return self._enabled
+
+    @enabled.setter
+    def enabled(self, on: bool) -> None:
+        self.launches = self.launches  # what the module counted so far, folded in
+        self._enabled = bool(on)
+
+    @property
+    def launches(self) -> int:
+        native = self._module.backward_launches() - self._native if self._enabled else 0
+        return self._called + native
+
+    @launches.setter
+    def launches(self, value: int) -> None:
+        self._called = value
+        self._native = self._module.backward_launches()
 
     def __getattr__(self, name):
         fn = getattr(self._module, name)
@@ -64,10 +89,11 @@ class _Counting:
             return fn
 
         def counted(*args, **kwargs):
-            if self.enabled:
-                self.launches += per
+            if self._enabled:
+                self._called += per
             return fn(*args, **kwargs)
 
+        setattr(self, name, counted)  # looked up once
         return counted
 
 

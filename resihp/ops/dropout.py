@@ -10,8 +10,6 @@ the reference, whose blocks have no dropout.)
 from __future__ import annotations
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _ext
 
@@ -58,25 +56,6 @@ def _signed(v: int) -> int:
     return v - (1 << 64) if v >> 63 else v
 
 
-class _Dropout(Function):
-    @staticmethod
-    def forward(ctx, x, residual, drop, seed, offset, state, first):
-        ctx.save_for_backward(*(() if state is None else (state,)))
-        ctx.args = (drop, seed, offset, first)
-        ctx.has_residual = residual is not None
-        return _ext.require().dropout(x, residual, drop, seed, offset, state, first)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        drop, seed, offset, first = ctx.args
-        state = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _ext.require().dropout(dout.contiguous(), None, drop, seed, offset, state, first)
-        return dx, (dout if ctx.has_residual else None), None, None, None, None, None
-
-
 def dropout(x, p: float, seed, offset: int = 0, residual=None, first_row: int = 0):
     """``x`` with a share ``p`` of its elements set to 0 and the others scaled, plus ``residual``.
 
@@ -108,8 +87,7 @@ def dropout(x, p: float, seed, offset: int = 0, residual=None, first_row: int = 
     if first_row < 0 or first + x.numel() >= 1 << 62:
         raise ValueError("first_row must not be negative, and indices must stay below 2**62")
     if x.is_cuda:
-        return _Dropout.apply(x.contiguous(), None if residual is None else residual.contiguous(),
-                              dropout_threshold(p), _signed(seed), _signed(offset), state, first)
+        return _ext.require().dropout_ad(x, dropout_threshold(p), _signed(seed), _signed(offset), first, state, residual)
     if state is not None:
         seed, offset = (int(v) % (1 << 64) for v in state)
     drop = dropout_threshold(p)

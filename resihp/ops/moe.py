@@ -24,11 +24,9 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _ext
-from .gemm import MAX_GROUPS, _cuda, check_groups, grouped_dgrad, grouped_wgrad
+from .gemm import MAX_GROUPS, _cuda, check_groups
 from .gemm import grouped_linear as _grouped_linear
 
 MAX_CHOICES = 16
@@ -75,22 +73,6 @@ def _route_torch(logits, k: int, normalize: bool):
     return weights, torch.where(allowed, ids, torch.full_like(ids, -1)).to(torch.int32)
 
 
-class _Route(Function):
-    @staticmethod
-    def forward(ctx, logits, k, normalize):
-        weights, ids, offsets, slots = _ext.require().moe_route(logits, k, normalize)
-        ctx.save_for_backward(logits, weights, ids)
-        ctx.normalize = normalize
-        ctx.mark_non_differentiable(ids, offsets, slots)
-        return weights, ids, offsets, slots
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dweights, *_):
-        logits, weights, ids = ctx.saved_tensors
-        return _ext.require().moe_route_bwd(logits, weights, ids, dweights.contiguous(), ctx.normalize), None, None
-
-
 def moe_route(logits, k: int, normalize: bool = True):
     """The ``k`` experts of every token: ``(weights, ids, plan)`` from router logits ``[T, E]``.
 
@@ -109,8 +91,7 @@ def moe_route(logits, k: int, normalize: bool = True):
         raise ValueError(f"{k} choices of {experts} experts: 1 to {MAX_CHOICES} choices, no more than experts, "
                          f"of 1 to {MAX_GROUPS} experts")
     if logits.is_cuda:
-        rows = logits if logits.stride(1) == 1 else logits.contiguous()
-        weights, ids, offsets, slots = _Route.apply(rows, int(k), bool(normalize))
+        weights, ids, offsets, slots = _ext.require().moe_route_ad(logits, k, normalize)
         return weights, ids, MoePlan(offsets, slots)
     weights, ids = _route_torch(logits, k, normalize)
     return weights, ids, _plan_torch(ids, experts, 0)
@@ -148,19 +129,6 @@ def _check_plan(rows, plan: MoePlan) -> tuple[torch.Tensor, torch.Tensor]:
     return offsets.contiguous(), slots.contiguous()
 
 
-class _Dispatch(Function):
-    @staticmethod
-    def forward(ctx, x, offsets, slots):
-        ctx.save_for_backward(offsets, slots)
-        return _ext.require().moe_scatter(x, offsets, slots)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        offsets, slots = ctx.saved_tensors
-        return _ext.require().moe_gather(dy.contiguous(), None, offsets, slots, None), None, None
-
-
 def moe_dispatch(x, plan: MoePlan):
     """Token rows ``x [T, d]`` in the plan's order ``[T * k, d]``: ``y[slots[t, j]] = x[t]``, zeros
     in the rows of choices that no expert takes."""
@@ -168,28 +136,10 @@ def moe_dispatch(x, plan: MoePlan):
     if x.shape[0] != slots.shape[0]:
         raise ValueError(f"{x.shape[0]} rows for a plan of {slots.shape[0]} tokens")
     if _cuda(x):
-        return _Dispatch.apply(x.contiguous(), offsets, slots)
+        return _ext.require().moe_dispatch_ad(x, offsets, slots)
     at = slots.long()
     rows = x[:, None, :] * (at < offsets[-1])[..., None].to(x.dtype)
     return torch.zeros_like(rows).view(-1, x.shape[1]).index_copy(0, at.reshape(-1), rows.reshape(-1, x.shape[1]))
-
-
-class _Combine(Function):
-    @staticmethod
-    def forward(ctx, y, weights, offsets, slots, residual):
-        ctx.save_for_backward(y, weights, offsets, slots)
-        ctx.has_residual = residual is not None
-        return _ext.require().moe_gather(y, weights, offsets, slots, residual)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        y, weights, offsets, slots = ctx.saved_tensors
-        dout = dout.contiguous()
-        dy = dw = None
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            dy, dw = _ext.require().moe_combine_bwd(dout, y, weights, offsets, slots)
-        return dy, dw, None, None, (dout if ctx.has_residual else None)
 
 
 def moe_combine(y, weights, plan: MoePlan, residual=None):
@@ -204,8 +154,7 @@ def moe_combine(y, weights, plan: MoePlan, residual=None):
                                  or residual.device != y.device):
         raise ValueError("the residual must be [T, d] in the rows' dtype, beside them")
     if _cuda(y):
-        return _Combine.apply(y.contiguous(), weights.contiguous(), offsets, slots,
-                              None if residual is None else residual.contiguous())
+        return _ext.require().moe_combine_ad(y, weights, offsets, slots, residual)
     at = slots.long()
     kept = (at < offsets[-1])[..., None]
     rows = torch.where(kept, y[at.reshape(-1)].view(*at.shape, -1), torch.zeros((), dtype=y.dtype, device=y.device))
@@ -216,27 +165,6 @@ def moe_combine(y, weights, plan: MoePlan, residual=None):
 # ---------------------------------------------------------------------------------------
 # per-expert linear layers
 # ---------------------------------------------------------------------------------------
-
-
-class _GroupedLinear(Function):
-    @staticmethod
-    def forward(ctx, x, w, offsets, main_grad):
-        ctx.save_for_backward(x, w, offsets)
-        ctx.main_grad = main_grad
-        return _grouped_linear(x, w, offsets)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w, offsets = ctx.saved_tensors
-        dy = dy.contiguous()
-        dx = grouped_dgrad(dy, w, offsets) if ctx.needs_input_grad[0] else None
-        dw = None
-        if ctx.main_grad is not None:
-            grouped_wgrad(dy, x, offsets, out=ctx.main_grad, accumulate=True)
-        elif ctx.needs_input_grad[1]:
-            dw = grouped_wgrad(dy, x, offsets).to(w.dtype)
-        return dx, dw, None, None
 
 
 def grouped_linear(x, w, offsets, main_grad=None):
@@ -253,4 +181,4 @@ def grouped_linear(x, w, offsets, main_grad=None):
         raise ValueError(f"main_grad must be a contiguous fp32 {list(w.shape)} beside the weights")
     if not _cuda(x):
         return _grouped_linear(x, w, offsets)
-    return _GroupedLinear.apply(x, w, offsets, main_grad)
+    return _ext.require().grouped_linear_ad(x, w, offsets.contiguous(), main_grad)
