@@ -200,9 +200,9 @@ void moe_plan(const int* ids, int64_t pairs, int start, int experts, int* counts
 void moe_scatter(const void* x, const int* slots, const int* used, void* out, int tokens, int k, int d, int* err,
                  cudaStream_t st);
 void moe_gather(const void* y, const float* weights, const void* residual, const int* slots, const int* used, void* out,
-                int tokens, int k, int d, int* err, cudaStream_t st);
+                int tokens, int k, int d, int* err, int num_sms, cudaStream_t st);
 void moe_combine_bwd(const void* dout, const void* y, const float* weights, const int* slots, const int* used, void* dy,
-                     float* dweights, int tokens, int k, int d, int* err, cudaStream_t st);
+                     float* dweights, int tokens, int k, int d, int* err, int num_sms, cudaStream_t st);
 
 // Products grouped by expert (grouped.cu): group g owns the rows offsets[g]..offsets[g + 1].
 struct GroupedShape {

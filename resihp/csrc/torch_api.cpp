@@ -406,7 +406,7 @@ torch::Tensor moe_gather_t(torch::Tensor y, c10::optional<torch::Tensor> weights
   c10::cuda::CUDAGuard guard(y.device());
   auto out = torch::empty({slots.size(0), y.size(1)}, y.options());
   moe_gather(y.data_ptr(), wp, rp, slots.data_ptr<int>(), offsets.data_ptr<int>() + offsets.numel() - 1, out.data_ptr(),
-             int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), cur_stream());
+             int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), sms(y), cur_stream());
   return out;
 }
 
@@ -422,7 +422,7 @@ std::vector<torch::Tensor> moe_combine_bwd_t(torch::Tensor dout, torch::Tensor y
   auto dw = torch::empty(slots.sizes(), y.options().dtype(torch::kFloat));
   moe_combine_bwd(dout.data_ptr(), y.data_ptr(), wp, slots.data_ptr<int>(),
                   offsets.data_ptr<int>() + offsets.numel() - 1, dy.data_ptr(), dw.data_ptr<float>(),
-                  int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), cur_stream());
+                  int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), sms(y), cur_stream());
   return {dy, dw};
 }
 
