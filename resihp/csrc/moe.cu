@@ -27,11 +27,6 @@ namespace {
 
 // ---- routing --------------------------------------------------------------------------
 
-// A row's logits in registers: 32 per lane leave room for half the warps.
-template <int VPT>
-constexpr int kRouteThreads = VPT > 8 ? 512 : 1024;
-constexpr int kBwdThreads = 256;
-
 // Unsigned order of the floats, both zeros alike, NaN above all, never 0.
 __device__ __forceinline__ uint32_t order_key(float v) {
   if (v != v) return 0xFFFFFFFFu;
@@ -50,149 +45,10 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
 }
 
-// LPR lanes share a row, lane l holds the logits l, l + LPR, ... Choice j ends up on lane j.
-// A choice is the largest key, then the lowest index that has it: two warp reductions on whole
-// warps, shuffles within the parts of a shared one.
-template <typename T, int LPR, int VPT>
-__global__ void __launch_bounds__(kRouteThreads<VPT>) route_kernel(const T* __restrict__ logits, int64_t ld, int tokens,
-                                                              int experts, int k, bool normalize, int rows_per_block,
-                                                              float* __restrict__ weights, int* __restrict__ ids,
-                                                              int* __restrict__ counts) {
-  pdl_enter();
-  extern __shared__ int hist[];  // [experts + 1]
-  for (int e = threadIdx.x; e <= experts; e += blockDim.x) hist[e] = 0;
-  __syncthreads();
-  constexpr int kRows = kRouteThreads<VPT> / LPR;
-  const int sub = threadIdx.x / LPR, lane = threadIdx.x % LPR;
-  const int first = blockIdx.x * rows_per_block;
-  const int last = min(tokens, first + rows_per_block);
-  // whole warps walk together (the reductions need every lane); rows past the end are idle
-  float ahead[VPT];  // the next row's logits, on their way during this row's reductions
-  auto fetch = [&](int row) {
-    #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      const int e = lane + v * LPR;
-      ahead[v] = row < last && e < experts ? logit_at(logits + int64_t(row) * ld + e) : -INFINITY;
-    }
-  };
-  fetch(first + sub);
-  for (int base = first; base < last; base += kRows) {
-    const int row = base + sub;
-    const bool live = row < last;
-    float x[VPT];
-    uint32_t key[VPT];
-    #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      x[v] = ahead[v];
-      key[v] = live && lane + v * LPR < experts ? order_key(x[v]) : 0u;
-    }
-    if (VPT <= 8) fetch(row + kRows);
-    float top = -INFINITY, mine = -INFINITY;
-    int id = -1;
-    for (int j = 0; j < k; ++j) {
-      uint32_t best = 0;
-      int at = 0;
-      #pragma unroll
-      for (int v = 0; v < VPT; ++v)
-        if (v == 0 || key[v] > best) { best = key[v]; at = lane + v * LPR; }
-      if (LPR == 32) {
-        const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, best);
-        at = int(__reduce_min_sync(0xFFFFFFFFu, best == most ? uint32_t(at) : 0xFFFFFFFFu));
-        best = most;
-      } else {
-        #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) {
-          const uint32_t ob = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-          const int oa = __shfl_xor_sync(0xFFFFFFFFu, at, o);
-          if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-        }
-      }
-      const bool allowed = best > kKeyNone;
-      if (j == 0 && allowed) top = key_value(best);
-      if (lane == j && allowed) { mine = key_value(best); id = at; }
-      #pragma unroll
-      for (int v = 0; v < VPT; ++v)
-        if (lane + v * LPR == at) key[v] = 0u;
-    }
-    const float m = top == -INFINITY ? 0.f : top;
-    const float num = id >= 0 ? expf(mine - m) : 0.f;
-    float sum = 0.f;
-    if (normalize) {
-      sum = num;
-    } else {
-      #pragma unroll
-      for (int v = 0; v < VPT; ++v) sum += expf(x[v] - m);
-    }
-    #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (live && lane < k) {
-      weights[int64_t(row) * k + lane] = id >= 0 ? num / sum : 0.f;
-      ids[int64_t(row) * k + lane] = id;
-      atomicAdd(&hist[id >= 0 ? id : experts], 1);
-    }
-    if (VPT > 8) fetch(row + kRows);
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e <= experts; e += blockDim.x) counts[int64_t(blockIdx.x) * (experts + 1) + e] = hist[e];
-}
-
-// d logit_e = sum_j w_j (1[e = id_j] - p_e) dw_j, p the softmax the weights came from. One
-// warp per row. The softmax over all experts needs no sums again: choice 0 is the largest
-// logit, so p_e = w_0 exp(l_e - l_{id_0}).
-template <typename T>
-__global__ void __launch_bounds__(kBwdThreads) route_bwd_kernel(const T* __restrict__ logits, int64_t ld,
-                                                                const float* __restrict__ weights,
-                                                                const int* __restrict__ ids,
-                                                                const float* __restrict__ dweights,
-                                                                T* __restrict__ dlogits, int tokens, int experts,
-                                                                int k, bool normalize) {
-  pdl_enter();
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * (kBwdThreads / 32) + (threadIdx.x >> 5);
-  if (row >= tokens) return;
-  int id = -1;
-  float w = 0.f, dw = 0.f;
-  if (lane < k) {
-    id = ids[int64_t(row) * k + lane];
-    w = weights[int64_t(row) * k + lane];
-    dw = dweights[int64_t(row) * k + lane];
-    if (id < 0) dw = 0.f;  // whatever arrives at a choice that was not made
-  }
-  float dot = w * dw;
-  #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
-  const float up = normalize ? w * (dw - dot) : w * dw;
-  const T* x = logits + int64_t(row) * ld;
-  const int id0 = __shfl_sync(0xFFFFFFFFu, id, 0);
-  const float w0 = __shfl_sync(0xFFFFFFFFu, w, 0);
-  const bool rest = !normalize && id0 >= 0 && id0 < experts;
-  const float x0 = rest ? logit_at(x + id0) : 0.f;
-  for (int e0 = 0; e0 < experts; e0 += 128) {  // four experts per lane
-    float g[4];
-    #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int e = e0 + v * 32 + lane;
-      g[v] = rest && e < experts ? -(w0 * expf(logit_at(x + e) - x0)) * dot : 0.f;
-    }
-    for (int j = 0; j < k; ++j) {
-      const int ej = __shfl_sync(0xFFFFFFFFu, id, j);
-      const float uj = __shfl_sync(0xFFFFFFFFu, up, j);
-      #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        if (e0 + v * 32 + lane == ej) g[v] += uj;
-    }
-    #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int e = e0 + v * 32 + lane;
-      if (e < experts) store_logit(dlogits + int64_t(row) * experts + e, g[v]);
-    }
-  }
-}
-
 // ---- plan -----------------------------------------------------------------------------
 
 // Expert of pair i in 0..experts-1, or ``experts`` for a pair that no expert here takes.
-__device__ __forceinline__ int expert_of(const int* __restrict__ ids, int64_t i, int start, int experts) {
+__device__ __forceinline__ int expert_of(const int* ids, int64_t i, int start, int experts) {
   const int64_t e = int64_t(ids[i]) - start;
   return e >= 0 && e < experts ? int(e) : experts;
 }
@@ -211,42 +67,20 @@ __global__ void __launch_bounds__(1024) plan_count_kernel(const int* __restrict_
   for (int e = threadIdx.x; e <= experts; e += blockDim.x) counts[int64_t(blockIdx.x) * (experts + 1) + e] = hist[e];
 }
 
-// Shared memory: place[experts + 1] (next place of each expert for this block) and
-// next[warps][experts + 1] (the same for each warp's run of the block's pairs).
-__global__ void __launch_bounds__(1024) plan_place_kernel(const int* __restrict__ ids, int64_t pairs,
-                                                          int64_t pairs_per_block, int start, int experts,
-                                                          const int* __restrict__ counts,
-                                                          int* __restrict__ offsets, int* __restrict__ slots) {
-  pdl_enter();
-  extern __shared__ int sm[];
+// The places of the pairs first .. last - 1 (per_block of them in every block but the last), by
+// one block. total[e]: all pairs of expert e; place[e]: those in the blocks before this one;
+// next: [warps][experts + 1] scratch. All in shared memory. Each warp takes a run of consecutive
+// pairs: it counts them, learns where its run starts within each expert, and hands out places
+// 32 pairs at a time, equal experts in lane order.
+__device__ __forceinline__ void place_pairs(const int* ids, int64_t first, int64_t last, int64_t per_block, int start,
+                                            int experts, int* total, int* place, int* next, int* offsets, int* slots) {
   const int width = experts + 1;
-  int* place = sm;
-  int* total = sm + width;
-  int* next = sm + 2 * width;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  for (int e = threadIdx.x; e < (2 + warps) * width; e += blockDim.x) sm[e] = 0;
+  for (int e = threadIdx.x; e < warps * width; e += blockDim.x) next[e] = 0;
   __syncthreads();
-  // this block's pairs, one contiguous run per warp
-  const int64_t first = blockIdx.x * pairs_per_block, last = min(pairs, first + pairs_per_block);
-  const int64_t per_warp = ((pairs_per_block + warps - 1) / warps + 31) / 32 * 32;
+  const int64_t per_warp = ((per_block + warps - 1) / warps + 31) / 32 * 32;
   const int64_t wfirst = first + warp * per_warp, wlast = min(last, wfirst + per_warp);
   for (int64_t i = wfirst + lane; i < wlast; i += 32) atomicAdd(&next[warp * width + expert_of(ids, i, start, experts)], 1);
-  const int cells = int(gridDim.x) * width;
-  constexpr int kBatch = 8;  // loads under way per thread: the counts come from L2
-  for (int c0 = threadIdx.x; c0 < cells; c0 += kBatch * blockDim.x) {
-    int v[kBatch];
-    #pragma unroll
-    for (int i = 0; i < kBatch; ++i) v[i] = c0 + i * int(blockDim.x) < cells ? counts[c0 + i * blockDim.x] : 0;
-    #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (v[i] == 0) continue;
-      const int c = c0 + i * int(blockDim.x);
-      const int b = c / width, e = c - b * width;
-      atomicAdd(&total[e], v[i]);
-      if (b < int(blockIdx.x)) atomicAdd(&place[e], v[i]);
-    }
-  }
-  __syncthreads();
   // exclusive sum of the totals over the experts, by one warp
   if (warp == 0) {
     int carry = 0;
@@ -287,6 +121,188 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(const int* __restrict_
       if (before == 0) mine[e] = at + __popc(same);
     }
     __syncwarp();
+  }
+}
+
+__global__ void __launch_bounds__(1024) plan_place_kernel(const int* __restrict__ ids, int64_t pairs,
+                                                          int64_t pairs_per_block, int start, int experts,
+                                                          const int* __restrict__ counts,
+                                                          int* __restrict__ offsets, int* __restrict__ slots) {
+  pdl_enter();
+  extern __shared__ int sm[];
+  const int width = experts + 1, blocks = int(gridDim.x), me = int(blockIdx.x);
+  int* total = sm;
+  int* place = sm + width;
+  for (int e = threadIdx.x; e < 2 * width; e += blockDim.x) sm[e] = 0;
+  __syncthreads();
+  // column sums of the blocks' counts: as many threads per expert as there are
+  const int parts = max(1, int(blockDim.x) / width);
+  for (int c = threadIdx.x; c < parts * width; c += blockDim.x) {
+    const int part = c / width, e = c - part * width;
+    int all = 0, before = 0;
+    #pragma unroll 8
+    for (int b = part; b < blocks; b += parts) {
+      const int v = counts[int64_t(b) * width + e];
+      all += v;
+      if (b < me) before += v;
+    }
+    atomicAdd(&total[e], all);
+    atomicAdd(&place[e], before);
+  }
+  const int64_t first = blockIdx.x * pairs_per_block;
+  place_pairs(ids, first, min(pairs, first + pairs_per_block), pairs_per_block, start, experts, total, place,
+              sm + 2 * width, offsets, slots);
+}
+
+// LPR lanes share a row, lane l holds the logits l, l + LPR, ...: eight to 32 per lane, so that
+// most of a choice is found within lanes and a warp serves 32 / LPR rows (a warp per row with
+// warp-wide reductions took 14 us for 32768 rows of 64 experts, four choices; this takes 9).
+// Lane j % LPR keeps choice j. A grid of one block goes on to sort its pairs itself.
+template <typename T, int LPR, int VPT, int KMAX>
+__global__ void __launch_bounds__(512) route_kernel(const T* __restrict__ logits, int64_t ld, int tokens, int experts,
+                                                    int k, bool normalize, int rows_per_block,
+                                                    float* __restrict__ weights, int* ids, int* __restrict__ counts,
+                                                    int* __restrict__ offsets, int* __restrict__ slots) {
+  pdl_enter();
+  extern __shared__ int sm[];
+  int* hist = sm;  // [experts + 1]
+  for (int e = threadIdx.x; e <= experts; e += blockDim.x) hist[e] = 0;
+  __syncthreads();
+  constexpr int kMine = (KMAX + LPR - 1) / LPR;  // choices a lane keeps: lane, lane + LPR, ...
+  const int rows = blockDim.x / LPR;
+  const int sub = threadIdx.x / LPR, lane = threadIdx.x % LPR;
+  const int first = blockIdx.x * rows_per_block;
+  const int last = min(tokens, first + rows_per_block);
+  // whole warps walk together (the shuffles need every lane); rows past the end are idle
+  for (int base = first; base < last; base += rows) {
+    const int row = base + sub;
+    const bool live = row < last;
+    float x[VPT];
+    uint32_t key[VPT];
+    #pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int e = lane + v * LPR;
+      x[v] = live && e < experts ? logit_at(logits + int64_t(row) * ld + e) : -INFINITY;
+    }
+    #pragma unroll
+    for (int v = 0; v < VPT; ++v) key[v] = live && lane + v * LPR < experts ? order_key(x[v]) : 0u;
+    float m = 0.f, mine[kMine];
+    int id[kMine];
+    #pragma unroll
+    for (int i = 0; i < kMine; ++i) id[i] = -1;
+    #pragma unroll 1
+    for (int j = 0; j < k; ++j) {
+      uint32_t best = key[0];
+      int at = lane;
+      #pragma unroll
+      for (int v = 1; v < VPT; ++v)
+        if (key[v] > best) { best = key[v]; at = lane + v * LPR; }
+      #pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) {
+        const uint32_t ob = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+        const int oa = __shfl_xor_sync(0xFFFFFFFFu, at, o);
+        if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
+      }
+      const bool allowed = best > kKeyNone;
+      const float value = key_value(best);
+      if (j == 0 && allowed) m = value;
+      #pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        if (lane + i * LPR == j && allowed) { mine[i] = value; id[i] = at; }
+      #pragma unroll
+      for (int v = 0; v < VPT; ++v)
+        if (lane + v * LPR == at) key[v] = 0u;
+    }
+    float sum = 0.f;
+    #pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      mine[i] = id[i] >= 0 ? expf(mine[i] - m) : 0.f;
+      if (normalize) sum += mine[i];
+    }
+    if (!normalize) {
+      #pragma unroll
+      for (int v = 0; v < VPT; ++v) sum += expf(x[v] - m);
+    }
+    #pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    #pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int j = lane + i * LPR;
+      if (live && j < k) {
+        weights[int64_t(row) * k + j] = id[i] >= 0 ? mine[i] / sum : 0.f;
+        ids[int64_t(row) * k + j] = id[i];
+        atomicAdd(&hist[id[i] >= 0 ? id[i] : experts], 1);
+      }
+    }
+  }
+  __syncthreads();
+  if (gridDim.x > 1) {
+    for (int e = threadIdx.x; e <= experts; e += blockDim.x)
+      counts[int64_t(blockIdx.x) * (experts + 1) + e] = hist[e];
+    return;
+  }
+  // one block: the totals are its own, and no pair comes before its first
+  int* place = sm + experts + 1;
+  for (int e = threadIdx.x; e <= experts; e += blockDim.x) place[e] = 0;
+  place_pairs(ids, 0, int64_t(tokens) * k, int64_t(tokens) * k, 0, experts, hist, place, place + experts + 1, offsets,
+              slots);
+}
+
+// d logit_e = sum_j w_j (1[e = id_j] - p_e) dw_j, p the softmax the weights came from. lpr lanes
+// per row, eight experts each at a time; every lane reads the row's choices, so nothing passes
+// between lanes. The softmax over all experts needs no sums again: choice 0 is the largest
+// logit, so p_e = w_0 exp(l_e - l_{id_0}).
+template <typename T, int KMAX>
+__global__ void __launch_bounds__(256) route_bwd_kernel(const T* __restrict__ logits, int64_t ld,
+                                                        const float* __restrict__ weights, const int* __restrict__ ids,
+                                                        const float* __restrict__ dweights, T* __restrict__ dlogits,
+                                                        int tokens, int experts, int k, bool normalize, int lpr) {
+  pdl_enter();
+  constexpr int kEach = 8;
+  const int row = blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  const int lane = threadIdx.x % lpr;
+  if (row >= tokens) return;
+  const T* x = logits + int64_t(row) * ld;
+  float l[kEach];
+  if (!normalize) {  // on their way while the choices arrive
+    #pragma unroll
+    for (int v = 0; v < kEach; ++v) l[v] = lane + v * lpr < experts ? logit_at(x + lane + v * lpr) : -INFINITY;
+  }
+  int id[KMAX];
+  float up[KMAX];
+  float dot = 0.f, w0 = 0.f;
+  #pragma unroll
+  for (int j = 0; j < KMAX; ++j) {
+    id[j] = -1;
+    up[j] = 0.f;
+    if (j < k) {
+      id[j] = ids[int64_t(row) * k + j];
+      const float w = weights[int64_t(row) * k + j];
+      if (j == 0) w0 = w;
+      // whatever arrives at a choice that was not made counts for nothing
+      if (id[j] >= 0) up[j] = w * dweights[int64_t(row) * k + j];
+      dot += up[j];
+    }
+  }
+  if (normalize) {
+    #pragma unroll
+    for (int j = 0; j < KMAX; ++j)
+      if (j < k && id[j] >= 0) up[j] -= weights[int64_t(row) * k + j] * dot;
+  }
+  const bool rest = !normalize && id[0] >= 0 && id[0] < experts;
+  const float x0 = rest ? logit_at(x + id[0]) : 0.f;
+  for (int e0 = 0; e0 < experts; e0 += kEach * lpr) {
+    #pragma unroll
+    for (int v = 0; v < kEach; ++v) {
+      const int e = e0 + lane + v * lpr;
+      if (e >= experts) break;
+      const float le = e0 == 0 || normalize ? l[v] : logit_at(x + e);
+      float g = rest ? -(w0 * expf(le - x0)) * dot : 0.f;
+      #pragma unroll
+      for (int j = 0; j < KMAX; ++j)
+        if (id[j] == e) g += up[j];
+      store_logit(dlogits + int64_t(row) * experts + e, g);
+    }
   }
 }
 
@@ -588,40 +604,62 @@ void launch_rows(void (*kernel)(MoveArgs, int), const MoveArgs& a, cudaStream_t 
   RESIHP_CUDA_CHECK(launch_pdl(kernel, grid, 256, 0, st, a, lpr));
 }
 
+// As many warps as their tables (and the block's two) leave within 48 KB: 16 up to 681 experts,
+// 9 at 1024.
+int place_warps(int experts, int most) { return std::min(most, 49152 / ((experts + 1) * int(sizeof(int))) - 2); }
+int place_bytes(int experts, int warps) { return (2 + warps) * (experts + 1) * int(sizeof(int)); }
+
 void launch_place(const int* ids, int64_t pairs, int64_t per_block, int blocks, int start, int experts,
                   const int* counts, int* offsets, int* slots, cudaStream_t st) {
-  // As many warps as their tables leave within 48 KB: 32 up to 360 experts, 9 at 1024.
-  const int table = (experts + 1) * int(sizeof(int));
-  const int warps = std::min(32, 49152 / table - 2);
-  RESIHP_CUDA_CHECK(launch_pdl(plan_place_kernel, blocks, 32 * warps, (2 + warps) * table, st, ids, pairs, per_block,
-                               start, experts, counts, offsets, slots));
+  const int warps = place_warps(experts, 16);
+  RESIHP_CUDA_CHECK(launch_pdl(plan_place_kernel, blocks, 32 * warps, place_bytes(experts, warps), st, ids, pairs,
+                               per_block, start, experts, counts, offsets, slots));
 }
 
-// Blocks of the counting sort: at least 1024 pairs each, at most one per SM (every block
-// reads every block's counts).
-int plan_blocks(int64_t pairs, int num_sms) { return std::max(1, std::min(num_sms, up(pairs, 1024))); }
+// Blocks of the counting sort: at least 512 pairs each, at most one per SM (every block reads
+// every block's counts).
+int plan_blocks(int64_t pairs, int num_sms) { return std::max(1, std::min(num_sms, up(pairs, 512))); }
+
+struct RouteCall {
+  const void* logits;
+  int64_t ld;
+  int tokens, experts, k;
+  bool normalize;
+  int rows_per_block, blocks;
+  float* weights;
+  int *ids, *counts, *offsets, *slots;
+};
 
 template <typename T, int LPR, int VPT>
-void launch_route_as(const void* logits, int64_t ld, int tokens, int experts, int k, bool normalize, int rows_per_block,
-                     int blocks, float* weights, int* ids, int* counts, cudaStream_t st) {
-  RESIHP_CUDA_CHECK(launch_pdl(route_kernel<T, LPR, VPT>, blocks, kRouteThreads<VPT>, (experts + 1) * int(sizeof(int)), st,
-                               static_cast<const T*>(logits), ld, tokens, experts, k, normalize, rows_per_block, weights,
-                               ids, counts));
+void launch_route_as(const RouteCall& c, cudaStream_t st) {
+  auto kernel = c.k <= 4 ? route_kernel<T, LPR, VPT, 4>
+                         : c.k <= 8 ? route_kernel<T, LPR, VPT, 8> : route_kernel<T, LPR, VPT, kMoeMaxChoices>;
+  const int warps = place_warps(c.experts, 16);
+  RESIHP_CUDA_CHECK(launch_pdl(kernel, c.blocks, 32 * warps, place_bytes(c.experts, warps), st,
+                               static_cast<const T*>(c.logits), c.ld, c.tokens, c.experts, c.k, c.normalize,
+                               c.rows_per_block, c.weights, c.ids, c.counts, c.offsets, c.slots));
 }
 
 template <typename T>
-void launch_route(const void* logits, int64_t ld, int tokens, int experts, int k, bool normalize, int rows_per_block,
-                  int blocks, float* weights, int* ids, int* counts, cudaStream_t st) {
-#define RESIHP_ROUTE(LPR, VPT) \
-  launch_route_as<T, LPR, VPT>(logits, ld, tokens, experts, k, normalize, rows_per_block, blocks, weights, ids, counts, st)
-  if (experts <= 8) RESIHP_ROUTE(8, 1);
-  else if (experts <= 16) RESIHP_ROUTE(16, 1);
-  else if (experts <= 32) RESIHP_ROUTE(32, 1);
-  else if (experts <= 64) RESIHP_ROUTE(32, 2);
-  else if (experts <= 128) RESIHP_ROUTE(32, 4);
-  else if (experts <= 256) RESIHP_ROUTE(32, 8);
-  else RESIHP_ROUTE(32, 32);
-#undef RESIHP_ROUTE
+void launch_route(const RouteCall& c, cudaStream_t st) {
+  if (c.experts <= 8) launch_route_as<T, 1, 8>(c, st);
+  else if (c.experts <= 16) launch_route_as<T, 2, 8>(c, st);
+  else if (c.experts <= 32) launch_route_as<T, 4, 8>(c, st);
+  else if (c.experts <= 64) launch_route_as<T, 8, 8>(c, st);
+  else if (c.experts <= 128) launch_route_as<T, 8, 16>(c, st);
+  else if (c.experts <= 256) launch_route_as<T, 16, 16>(c, st);
+  else if (c.experts <= 512) launch_route_as<T, 32, 16>(c, st);
+  else launch_route_as<T, 32, 32>(c, st);
+}
+
+template <typename T>
+void launch_route_bwd(const void* logits, int64_t ld, const float* weights, const int* ids, const float* dweights,
+                      void* dlogits, int tokens, int experts, int k, bool normalize, cudaStream_t st) {
+  int lpr = 1;
+  while (lpr < 32 && lpr * 8 < experts) lpr <<= 1;
+  auto kernel = k <= 4 ? route_bwd_kernel<T, 4> : k <= 8 ? route_bwd_kernel<T, 8> : route_bwd_kernel<T, kMoeMaxChoices>;
+  RESIHP_CUDA_CHECK(launch_pdl(kernel, up(tokens, 256 / lpr), 256, 0, st, static_cast<const T*>(logits), ld, weights,
+                               ids, dweights, static_cast<T*>(dlogits), tokens, experts, k, normalize, lpr));
 }
 
 }  // namespace
@@ -637,23 +675,18 @@ void moe_route(const void* logits, bool bf16, int64_t ld, int tokens, int expert
   const int64_t pairs = int64_t(tokens) * k;
   const int rows_per_block = std::max(1, up(tokens, plan_blocks(pairs, num_sms)));
   const int blocks = std::max(1, up(tokens, rows_per_block));
-  if (bf16) launch_route<__nv_bfloat16>(logits, ld, tokens, experts, k, normalize, rows_per_block, blocks, weights, ids, counts, st);
-  else launch_route<float>(logits, ld, tokens, experts, k, normalize, rows_per_block, blocks, weights, ids, counts, st);
-  launch_place(ids, pairs, int64_t(rows_per_block) * k, blocks, 0, experts, counts, offsets, slots, st);
+  const RouteCall c{logits, ld, tokens, experts, k, normalize, rows_per_block, blocks, weights, ids, counts, offsets, slots};
+  if (bf16) launch_route<__nv_bfloat16>(c, st);
+  else launch_route<float>(c, st);
+  if (blocks > 1) launch_place(ids, pairs, int64_t(rows_per_block) * k, blocks, 0, experts, counts, offsets, slots, st);
 }
 
 void moe_route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* ids,
                    const float* dweights, void* dlogits, int tokens, int experts, int k, bool normalize,
                    cudaStream_t st) {
   if (tokens == 0) return;
-  const int grid = up(tokens, kBwdThreads / 32);
-  if (bf16)
-    RESIHP_CUDA_CHECK(launch_pdl(route_bwd_kernel<__nv_bfloat16>, grid, kBwdThreads, 0, st,
-                                 static_cast<const __nv_bfloat16*>(logits), ld, weights, ids, dweights,
-                                 static_cast<__nv_bfloat16*>(dlogits), tokens, experts, k, normalize));
-  else
-    RESIHP_CUDA_CHECK(launch_pdl(route_bwd_kernel<float>, grid, kBwdThreads, 0, st, static_cast<const float*>(logits),
-                                 ld, weights, ids, dweights, static_cast<float*>(dlogits), tokens, experts, k, normalize));
+  if (bf16) launch_route_bwd<__nv_bfloat16>(logits, ld, weights, ids, dweights, dlogits, tokens, experts, k, normalize, st);
+  else launch_route_bwd<float>(logits, ld, weights, ids, dweights, dlogits, tokens, experts, k, normalize, st);
 }
 
 void moe_plan(const int* ids, int64_t pairs, int start, int experts, int* counts, int* offsets, int* slots, int num_sms,
