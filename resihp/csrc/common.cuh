@@ -30,7 +30,7 @@ enum ErrorCode : int {
   kErrMmaWait = 2,      // MMA issuer waited too long for a filled stage / free accumulator
   kErrEpiWait = 3,      // epilogue waited too long for a finished accumulator
   kErrPeerWait = 4,     // a cross-GPU flag never arrived
-  kErrBounds = 5,       // a bounds check in a checked build skipped an access
+  kErrBounds = 5,       // a bounds check skipped or clamped an access
 };
 
 __device__ __forceinline__ uint64_t globaltimer() {

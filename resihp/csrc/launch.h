@@ -188,9 +188,11 @@ void dropout(const void* x, const void* residual, void* out, bool bf16, int64_t 
 // moe_blocks(tokens * k) x (experts + 1) ints.
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxChoices = 16;
+constexpr int kMoeMaxPairs = 0x7FFF0000;  // tokens * k: leaves room for a block's rows in 31 bits
 int moe_blocks(int64_t pairs, int num_sms);
-void moe_route(const void* logits, bool bf16, int64_t ld, int tokens, int experts, int k, bool normalize,
-               float* weights, int* ids, int* counts, int* offsets, int* slots, int num_sms, cudaStream_t st);
+// (returns how many kernels it launched)
+int moe_route(const void* logits, bool bf16, int64_t ld, int tokens, int experts, int k, bool normalize,
+              float* weights, int* ids, int* counts, int* offsets, int* slots, int num_sms, cudaStream_t st);
 void moe_route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* ids,
                    const float* dweights, void* dlogits, int tokens, int experts, int k, bool normalize,
                    cudaStream_t st);

@@ -14,8 +14,12 @@
 // pairs warp by warp and writes their places. Nothing is decided by the order of atomics
 // (they only count), so a plan is the same on every run; and no state outlives a call.
 //
-// Both row movements go token by token, so a token's row is read (or written) once however
-// many experts it has: k + 1 rows move per token, which is all that has to move.
+// The row movements go by token (or by pair, one token's pairs side by side), so a token's row
+// comes from memory once however many experts it has: k + 1 rows move per token, which is all
+// that has to move. They are bound by memory: at 4096 tokens of two choices, width 2048, dispatch
+// takes 7.0 us, combine 11.4, their gradients 8.4 and 13.5, at 5.9 TB/s and more of the 6.5 a
+// copy reaches. Rows of an odd width have no common alignment and move two bytes at a time: 1021
+// tokens of six choices, width 1003, take 5.6 us out and 9.0 back, where their bytes take 2.2.
 #include <algorithm>
 
 #include "common.cuh"
@@ -308,6 +312,7 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const T* __restrict__ lo
 
 // ---- row movements --------------------------------------------------------------------
 
+// A row as 16-byte vectors, or element by element where its width or address forbids them.
 template <int VEC>
 struct Row;
 template <>
@@ -459,8 +464,8 @@ __global__ void __launch_bounds__(256) gather_warp_kernel(MoveArgs a) {
       float w[J];
       #pragma unroll
       for (int j = 0; j < J; ++j) {
-        s[j] = __shfl_sync(0xFFFFFFFFu, place, (j0 + j) & 31);  // lanes from k on hold none
-        w[j] = __shfl_sync(0xFFFFFFFFu, weight, (j0 + j) & 31);
+        s[j] = __shfl_sync(0xFFFFFFFFu, place, j0 + j);  // lanes from k on hold none (k even or below 32)
+        w[j] = __shfl_sync(0xFFFFFFFFu, weight, j0 + j);
         #pragma unroll
         for (int u = 0; u < U; ++u)
           if (s[j] >= 0 && v + u * 32 < vpr) raw[j][u] = static_cast<const Raw*>(a.in)[int64_t(s[j]) * vpr + v + u * 32];
@@ -593,7 +598,7 @@ bool vectors(const MoveArgs& a) {
 
 void check_move(const MoveArgs& a) {
   RESIHP_CHECK(a.k >= 1 && a.d >= 1 && a.tokens >= 0, "moe rows: sizes must be positive");
-  RESIHP_CHECK(int64_t(a.tokens) * a.k <= INT32_MAX, "moe rows: tokens * k passes 31 bits");
+  RESIHP_CHECK(int64_t(a.tokens) * a.k <= kMoeMaxPairs, "moe rows: tokens * k passes ", kMoeMaxPairs);
 }
 
 template <int VEC, int U>
@@ -630,15 +635,29 @@ struct RouteCall {
   int *ids, *counts, *offsets, *slots;
 };
 
-template <typename T, int LPR, int VPT>
+template <typename T, int LPR, int VPT, int KMAX>
 void launch_route_as(const RouteCall& c, cudaStream_t st) {
-  auto kernel = c.k <= 4 ? route_kernel<T, LPR, VPT, 4>
-                         : c.k <= 8 ? route_kernel<T, LPR, VPT, 8> : route_kernel<T, LPR, VPT, kMoeMaxChoices>;
   const int warps = place_warps(c.experts, 16);
-  RESIHP_CUDA_CHECK(launch_pdl(kernel, c.blocks, 32 * warps, place_bytes(c.experts, warps), st,
+  RESIHP_CUDA_CHECK(launch_pdl(route_kernel<T, LPR, VPT, KMAX>, c.blocks, 32 * warps, place_bytes(c.experts, warps), st,
                                static_cast<const T*>(c.logits), c.ld, c.tokens, c.experts, c.k, c.normalize,
                                c.rows_per_block, c.weights, c.ids, c.counts, c.offsets, c.slots));
 }
+
+// By the choices that a lane has to keep.
+template <typename T, int LPR, int VPT>
+void launch_route_as(const RouteCall& c, cudaStream_t st) {
+  if constexpr (LPR >= 16) {
+    launch_route_as<T, LPR, VPT, 16>(c, st);
+  } else if constexpr (LPR == 8) {
+    if (c.k <= 8) launch_route_as<T, LPR, VPT, 8>(c, st);
+    else launch_route_as<T, LPR, VPT, 16>(c, st);
+  } else {
+    if (c.k <= 4) launch_route_as<T, LPR, VPT, 4>(c, st);
+    else if (c.k <= 8) launch_route_as<T, LPR, VPT, 8>(c, st);
+    else launch_route_as<T, LPR, VPT, 16>(c, st);
+  }
+}
+static_assert(kMoeMaxChoices == 16, "the router keeps up to 16 choices");
 
 template <typename T>
 void launch_route(const RouteCall& c, cudaStream_t st) {
@@ -666,19 +685,21 @@ void launch_route_bwd(const void* logits, int64_t ld, const float* weights, cons
 
 int moe_blocks(int64_t pairs, int num_sms) { return plan_blocks(pairs, num_sms); }
 
-void moe_route(const void* logits, bool bf16, int64_t ld, int tokens, int experts, int k, bool normalize,
+int moe_route(const void* logits, bool bf16, int64_t ld, int tokens, int experts, int k, bool normalize,
                float* weights, int* ids, int* counts, int* offsets, int* slots, int num_sms, cudaStream_t st) {
   RESIHP_CHECK(experts >= 1 && experts <= kMoeMaxExperts, "moe_route takes 1 to ", kMoeMaxExperts, " experts");
   RESIHP_CHECK(k >= 1 && k <= kMoeMaxChoices && k <= experts, "moe_route takes 1 to ", kMoeMaxChoices,
                " choices, no more than experts");
-  RESIHP_CHECK(int64_t(tokens) * k <= INT32_MAX, "moe_route: tokens * k passes 31 bits");
+  RESIHP_CHECK(int64_t(tokens) * k <= kMoeMaxPairs, "moe_route: tokens * k passes ", kMoeMaxPairs);
   const int64_t pairs = int64_t(tokens) * k;
   const int rows_per_block = std::max(1, up(tokens, plan_blocks(pairs, num_sms)));
   const int blocks = std::max(1, up(tokens, rows_per_block));
   const RouteCall c{logits, ld, tokens, experts, k, normalize, rows_per_block, blocks, weights, ids, counts, offsets, slots};
   if (bf16) launch_route<__nv_bfloat16>(c, st);
   else launch_route<float>(c, st);
-  if (blocks > 1) launch_place(ids, pairs, int64_t(rows_per_block) * k, blocks, 0, experts, counts, offsets, slots, st);
+  if (blocks == 1) return 1;
+  launch_place(ids, pairs, int64_t(rows_per_block) * k, blocks, 0, experts, counts, offsets, slots, st);
+  return 2;
 }
 
 void moe_route_bwd(const void* logits, bool bf16, int64_t ld, const float* weights, const int* ids,
@@ -692,7 +713,7 @@ void moe_route_bwd(const void* logits, bool bf16, int64_t ld, const float* weigh
 void moe_plan(const int* ids, int64_t pairs, int start, int experts, int* counts, int* offsets, int* slots, int num_sms,
               cudaStream_t st) {
   RESIHP_CHECK(experts >= 1 && experts <= kMoeMaxExperts, "moe_plan takes 1 to ", kMoeMaxExperts, " experts");
-  RESIHP_CHECK(pairs <= INT32_MAX, "moe_plan: tokens * k passes 31 bits");
+  RESIHP_CHECK(pairs <= kMoeMaxPairs, "moe_plan: tokens * k passes ", kMoeMaxPairs);
   const int64_t per_block = std::max(1, up(pairs, plan_blocks(pairs, num_sms)));
   const int blocks = std::max(1, up(pairs, per_block));
   RESIHP_CUDA_CHECK(launch_pdl(plan_count_kernel, blocks, 1024, (experts + 1) * int(sizeof(int)), st, ids, pairs,
@@ -717,7 +738,7 @@ void moe_gather(const void* y, const float* weights, const void* residual, const
   const bool many = tokens >= num_sms * 16;
   if (!vectors(a)) {
     launch_rows<1, 4>(gather_kernel<1, 4, kTogether>, a, st);
-  } else if (many && d >= 256) {
+  } else if (many && d >= 256 && k <= 32) {  // (a lane of the warp holds a choice's place)
     RESIHP_CUDA_CHECK(launch_pdl(gather_warp_kernel<8, 2, 2>, up(tokens, 8), 256, 0, st, a));
   } else {
     launch_rows<8, 1>(many ? gather_kernel<8, 1, 1> : gather_kernel<8, 1, kTogether>, a, st);

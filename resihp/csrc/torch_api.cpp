@@ -282,6 +282,13 @@ torch::Tensor attn_bwd_t(torch::Tensor qkv, torch::Tensor out, torch::Tensor dou
 }
 
 
+// ---- launch count -----------------------------------------------------------------------
+// Kernels launched by the calls below, those of backward passes included, which no Python call
+// shows (the launch counter adds them to what it sees).
+
+static std::atomic<int64_t> g_launches{0};
+static void count_launches(int64_t n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
+
 // ---- dropout --------------------------------------------------------------------------
 
 torch::Tensor dropout_t(torch::Tensor x, c10::optional<torch::Tensor> residual, int64_t drop, int64_t seed,
@@ -306,6 +313,7 @@ torch::Tensor dropout_t(torch::Tensor x, c10::optional<torch::Tensor> residual, 
   auto out = torch::empty_like(x);
   dropout(x.data_ptr(), rp, out.data_ptr(), x.scalar_type() == at::kBFloat16, x.numel(), first, uint64_t(seed),
           uint64_t(offset), sp, uint32_t(drop), sms(x), cur_stream());
+  count_launches(x.numel() > 0);
   return out;
 }
 
@@ -317,7 +325,7 @@ static void check_int32(const torch::Tensor& t, const torch::Tensor& like, const
 }
 
 static void check_rows_count(int64_t rows, int64_t k) {
-  TORCH_CHECK(rows * k <= INT32_MAX, "tokens * k passes 31 bits");
+  TORCH_CHECK(rows <= kMoeMaxPairs / std::max<int64_t>(k, 1), "tokens * k passes ", kMoeMaxPairs);
 }
 
 std::vector<torch::Tensor> moe_route_t(torch::Tensor logits, int64_t k, bool normalize) {
@@ -332,9 +340,9 @@ std::vector<torch::Tensor> moe_route_t(torch::Tensor logits, int64_t k, bool nor
   auto slots = torch::empty({t, k}, ints);
   auto offsets = torch::empty({e + 1}, ints);
   auto counts = torch::empty({moe_blocks(t * k, sms(logits)), e + 1}, ints);
-  moe_route(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0), int(t), int(e), int(k), normalize,
-            weights.data_ptr<float>(), ids.data_ptr<int>(), counts.data_ptr<int>(), offsets.data_ptr<int>(),
-            slots.data_ptr<int>(), sms(logits), cur_stream());
+  count_launches(moe_route(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0), int(t), int(e),
+                           int(k), normalize, weights.data_ptr<float>(), ids.data_ptr<int>(), counts.data_ptr<int>(),
+                           offsets.data_ptr<int>(), slots.data_ptr<int>(), sms(logits), cur_stream()));
   return {weights, ids, offsets, slots};
 }
 
@@ -348,6 +356,7 @@ torch::Tensor moe_route_bwd_t(torch::Tensor logits, torch::Tensor weights, torch
   moe_route_bwd(logits.data_ptr(), logits.scalar_type() == at::kBFloat16, logits.stride(0), weights.data_ptr<float>(),
                 ids.data_ptr<int>(), dweights.data_ptr<float>(), out.data_ptr(), int(t), int(e), int(k), normalize,
                 cur_stream());
+  count_launches(t > 0);
   return out;
 }
 
@@ -362,6 +371,7 @@ std::vector<torch::Tensor> moe_plan_t(torch::Tensor ids, int64_t experts, int64_
   auto counts = torch::empty({moe_blocks(ids.numel(), sms(ids)), experts + 1}, ids.options());
   moe_plan(ids.data_ptr<int>(), ids.numel(), int(start), int(experts), counts.data_ptr<int>(), offsets.data_ptr<int>(),
            slots.data_ptr<int>(), sms(ids), cur_stream());
+  count_launches(2);
   return {offsets, slots};
 }
 
@@ -381,6 +391,7 @@ torch::Tensor moe_scatter_t(torch::Tensor x, torch::Tensor offsets, torch::Tenso
   auto out = torch::empty({slots.numel(), x.size(1)}, x.options());
   moe_scatter(x.data_ptr(), slots.data_ptr<int>(), offsets.data_ptr<int>() + offsets.numel() - 1, out.data_ptr(),
               int(x.size(0)), int(slots.size(1)), int(x.size(1)), error_word(x.device()), cur_stream());
+  count_launches(x.size(0) > 0);
   return out;
 }
 
@@ -407,6 +418,7 @@ torch::Tensor moe_gather_t(torch::Tensor y, c10::optional<torch::Tensor> weights
   auto out = torch::empty({slots.size(0), y.size(1)}, y.options());
   moe_gather(y.data_ptr(), wp, rp, slots.data_ptr<int>(), offsets.data_ptr<int>() + offsets.numel() - 1, out.data_ptr(),
              int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), sms(y), cur_stream());
+  count_launches(slots.size(0) > 0);
   return out;
 }
 
@@ -423,6 +435,7 @@ std::vector<torch::Tensor> moe_combine_bwd_t(torch::Tensor dout, torch::Tensor y
   moe_combine_bwd(dout.data_ptr(), y.data_ptr(), wp, slots.data_ptr<int>(),
                   offsets.data_ptr<int>() + offsets.numel() - 1, dy.data_ptr(), dw.data_ptr<float>(),
                   int(slots.size(0)), int(slots.size(1)), int(y.size(1)), error_word(y.device()), sms(y), cur_stream());
+  count_launches(slots.size(0) > 0);
   return {dy, dw};
 }
 
@@ -448,6 +461,7 @@ torch::Tensor grouped_rows_t(torch::Tensor a, torch::Tensor w, bool w_mn, torch:
   auto c = torch::empty({a.size(0), n}, a.options());
   grouped_rows(a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(1), w.stride(0), w_mn, c.data_ptr(), n, s,
                error_word(a.device()), cur_stream());
+  count_launches(s.rows > 0);
   return c;
 }
 
@@ -463,6 +477,7 @@ void grouped_wgrad_t(torch::Tensor dy, torch::Tensor x, torch::Tensor offsets, t
   c10::cuda::CUDAGuard guard(dy.device());
   grouped_wgrad(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), out.data_ptr<float>(), accumulate, s,
                 error_word(dy.device()), cur_stream());
+  count_launches(s.rows > 0);
 }
 
 // ---- differentiable forms -------------------------------------------------------------------
@@ -475,13 +490,12 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = c10::optional<torch::Tensor>;
 
-// Kernels launched by backward passes (the launch counter adds them to what Python calls).
-static std::atomic<int64_t> g_backward_launches{0};
-static void count_backward(int64_t n) { g_backward_launches.fetch_add(n, std::memory_order_relaxed); }
 
 // These gradients have no derivative of their own: asking for one raises.
 static variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);  // or the error's node would not be recorded
   auto error = std::make_shared<torch::autograd::DelayedError>(
       "trying to differentiate twice an operator of resihp whose gradient has no derivative", int64_t(grads.size()));
   return (*error)(std::move(grads));
@@ -501,10 +515,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     OptTensor state;
     if (a[5]) state = ctx->get_saved_variables()[0];
     torch::Tensor dx;
-    if (ctx->needs_input_grad(0)) {
-      dx = dropout_t(grads[0].contiguous(), c10::nullopt, a[0], a[1], a[2], state, a[3]);
-      count_backward(1);
-    }
+    if (ctx->needs_input_grad(0)) dx = dropout_t(grads[0].contiguous(), c10::nullopt, a[0], a[1], a[2], state, a[3]);
     return once({dx, {}, {}, {}, {}, {}, a[4] ? grads[0] : torch::Tensor()});
   }
 };
@@ -522,7 +533,6 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}, {}};
     const auto saved = ctx->get_saved_variables();
-    count_backward(1);
     return once({moe_route_bwd_t(saved[0], saved[1], saved[2], grads[0].contiguous(),
                                  ctx->saved_data["normalize"].toBool()), {}, {}});
   }
@@ -536,7 +546,6 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    count_backward(1);
     return once({moe_gather_t(grads[0].contiguous(), c10::nullopt, saved[0], saved[1], c10::nullopt), {}, {}});
   }
 };
@@ -553,10 +562,8 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     std::vector<torch::Tensor> d(2);
-    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
+    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1))
       d = moe_combine_bwd_t(grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3]);
-      count_backward(1);
-    }
     return once({d[0], d[1], {}, {}, ctx->saved_data["residual"].toBool() ? grads[0] : torch::Tensor()});
   }
 };
@@ -581,18 +588,13 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     const auto saved = ctx->get_saved_variables();
     const auto dy = tiles_of(grads[0]);
     torch::Tensor dx, dw;
-    if (ctx->needs_input_grad(0)) {
-      dx = grouped_rows_t(dy, saved[1], true, saved[2]);
-      count_backward(1);
-    }
+    if (ctx->needs_input_grad(0)) dx = grouped_rows_t(dy, saved[1], true, saved[2]);
     const auto acc = ctx->saved_data.find("main_grad");
     if (acc != ctx->saved_data.end()) {
       grouped_wgrad_t(dy, saved[0], saved[2], acc->second.toTensor(), true);
-      count_backward(1);
     } else if (ctx->needs_input_grad(1)) {
       auto sum = torch::empty(saved[1].sizes(), saved[1].options().dtype(torch::kFloat));
       grouped_wgrad_t(dy, saved[0], saved[2], sum, false);
-      count_backward(1);
       dw = sum.to(saved[1].scalar_type());
     }
     return once({dx, dw, {}, {}});
@@ -856,8 +858,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_combine_bwd", &resihp::moe_combine_bwd_t);
   m.def("grouped_rows", &resihp::grouped_rows_t);
   m.def("grouped_wgrad", &resihp::grouped_wgrad_t);
-  m.def("backward_launches", [] { return resihp::g_backward_launches.load(); },
-        "kernels launched so far by the backward passes of the differentiable forms below");
+  m.def("native_launches", [] { return resihp::g_launches.load(); },
+        "kernels launched so far by the calls from dropout to grouped_linear_ad, backward passes included");
   m.def("dropout_ad", &resihp::dropout_ad);
   m.def("moe_route_ad", &resihp::moe_route_ad);
   m.def("moe_dispatch_ad", &resihp::moe_dispatch_ad);

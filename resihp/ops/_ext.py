@@ -43,9 +43,6 @@ def _load():
 KERNELS_PER_CALL = {
     "gemm": 1, "rmsnorm_fwd": 1, "rmsnorm_bwd": 2, "rope": 1, "swiglu_fwd": 1, "swiglu_bwd": 1,
     "adamw": 1, "embedding_fwd": 1, "embedding_bwd": 2, "xent_stats": 1, "xent_grad": 1,
-    "dropout": 1, "moe_route": 2, "moe_route_bwd": 1, "moe_plan": 2, "moe_scatter": 1, "moe_gather": 1,
-    "moe_combine_bwd": 1, "grouped_rows": 1, "grouped_wgrad": 1,
-    "dropout_ad": 1, "moe_route_ad": 2, "moe_dispatch_ad": 1, "moe_combine_ad": 1, "grouped_linear_ad": 1,
     "attn_fwd": 1, "attn_bwd": 3, "ag_gemm": 1, "gemm_rs": 1, "dp_allreduce_adamw": 1, "reshard_gather": 1,
 }
 
@@ -53,8 +50,8 @@ KERNELS_PER_CALL = {
 class _Counting:
     """Proxy over the extension module that counts kernel launches per entry point.
 
-    The ``*_ad`` entry points launch their backward kernels from C++, where Python does not see
-    them: the module counts those itself.
+    Entry points whose backward passes run in C++ (dropout, the sparse MLP) are counted by the
+    module itself: Python does not see every launch of theirs.
     """
 
     def __init__(self, module):
@@ -74,13 +71,13 @@ class _Counting:
 
     @property
     def launches(self) -> int:
-        native = self._module.backward_launches() - self._native if self._enabled else 0
+        native = self._module.native_launches() - self._native if self._enabled else 0
         return self._called + native
 
     @launches.setter
     def launches(self, value: int) -> None:
         self._called = value
-        self._native = self._module.backward_launches()
+        self._native = self._module.native_launches()
 
     def __getattr__(self, name):
         fn = getattr(self._module, name)

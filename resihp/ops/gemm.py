@@ -194,7 +194,7 @@ ERROR_CODES = {
     2: "MMA issuer waited past its budget for a filled stage or a free accumulator",
     3: "epilogue waited past its budget for a finished accumulator",
     4: "a wait on another GPU's flag ran out its budget (peer never arrived)",
-    5: "a bounds check of the checked build skipped an access",
+    5: "a bounds check skipped an access (offsets or places of a sparse MLP out of range, or the checked build)",
 }
 PEER_WAIT = 4
 

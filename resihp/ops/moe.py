@@ -37,7 +37,9 @@ class MoePlan(NamedTuple):
 
     ``offsets`` (int32 ``[E + 1]``): expert ``e`` owns the rows ``offsets[e] .. offsets[e + 1]``.
     ``slots`` (int32 ``[T, k]``): each pair's row; pairs of no expert have the rows from
-    ``offsets[E]`` on. Every row belongs to exactly one pair.
+    ``offsets[E]`` on. Every row belongs to exactly one pair; a plan made elsewhere has to keep
+    that (of two pairs with one place either may win). Places outside the rows are left out,
+    and on the kernels reported by :func:`resihp.ops.check_device_errors`.
     """
 
     offsets: torch.Tensor
@@ -137,9 +139,12 @@ def moe_dispatch(x, plan: MoePlan):
         raise ValueError(f"{x.shape[0]} rows for a plan of {slots.shape[0]} tokens")
     if _cuda(x):
         return _ext.require().moe_dispatch_ad(x, offsets, slots)
-    at = slots.long()
-    rows = x[:, None, :] * (at < offsets[-1])[..., None].to(x.dtype)
-    return torch.zeros_like(rows).view(-1, x.shape[1]).index_copy(0, at.reshape(-1), rows.reshape(-1, x.shape[1]))
+    at = slots.long().reshape(-1)
+    count = at.numel()
+    kept = (at < offsets[-1])[:, None]
+    rows = torch.where(kept, x.repeat_interleave(slots.shape[1], 0), torch.zeros((), dtype=x.dtype, device=x.device))
+    at = torch.where((at >= 0) & (at < count), at, torch.full_like(at, count))  # places out of range go nowhere
+    return x.new_zeros(count + 1, x.shape[1]).index_copy(0, at, rows)[:count]
 
 
 def moe_combine(y, weights, plan: MoePlan, residual=None):
@@ -156,9 +161,10 @@ def moe_combine(y, weights, plan: MoePlan, residual=None):
     if _cuda(y):
         return _ext.require().moe_combine_ad(y, weights, offsets, slots, residual)
     at = slots.long()
-    kept = (at < offsets[-1])[..., None]
-    rows = torch.where(kept, y[at.reshape(-1)].view(*at.shape, -1), torch.zeros((), dtype=y.dtype, device=y.device))
-    out = (rows * weights[..., None]).sum(1)
+    kept = ((at >= 0) & (at < offsets[-1].clamp_max(at.numel())))[..., None]
+    rows = y[torch.where(kept[..., 0], at, torch.zeros_like(at)).reshape(-1)].view(*at.shape, -1) if at.numel() else \
+        y.new_zeros(*at.shape, y.shape[1])
+    out = (torch.where(kept, rows, torch.zeros((), dtype=y.dtype, device=y.device)) * weights[..., None]).sum(1)
     return out if residual is None else residual + out
 
 

@@ -229,3 +229,31 @@ def test_recomputed_activations_drop_the_same_elements():
     z = x.detach().clone().requires_grad_()
     layer(z).backward(torch.ones_like(y))
     assert torch.equal(x.grad, z.grad)
+
+
+@gpu
+def test_gradient_has_no_second_derivative():
+    x = torch.randn(4, 16, device="cuda").bfloat16().requires_grad_()
+    (dx,) = torch.autograd.grad(fn.dropout(x, 0.5, 1).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dx.float().sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_against_differences(dtype):
+    """Dropout is linear: the difference of two inputs that are apart by h in one element equals
+    the gradient times h, up to the outputs' roundings."""
+    x = torch.randn(9, 24, device="cuda").to(dtype)
+    h = 0.5
+    keep = dropout_mask(216, 0.25, 3, 4).view(9, 24)
+    leaf = x.clone().requires_grad_()
+    fn.dropout(leaf, 0.25, 3, 4).backward(torch.ones_like(x))
+    for r, c in ((0, 0), (3, 7), (8, 23)):
+        moved = x.clone()
+        moved[r, c] += h
+        step = (moved - x)[r, c].double().item()
+        diff = (fn.dropout(moved, 0.25, 3, 4) - fn.dropout(x, 0.25, 3, 4)).double().sum().item()
+        size = abs(moved[r, c].item()) + abs(x[r, c].item())
+        assert abs(diff - leaf.grad[r, c].item() * step) <= 4 * HALF[dtype] * (size + h) * 65536 / (65536 - 16384)
+        assert (leaf.grad[r, c] != 0).item() == keep[r, c].item()

@@ -749,3 +749,165 @@ def test_rows_far_into_memory():
     want = x[-1].double() * 0.125 * 6  # the last token's last two choices have no expert
     near(out[-1], want, BF * want.abs() + 20 * F32 * want.abs())
     check_device_errors()
+
+
+# ---------------------------------------------------------------------------------------
+# GPU: calls that the documentation allows and nothing above makes
+# ---------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("t,k,d", [(5000, 40, 256), (5000, 31, 264), (5000, 32, 256), (9, 40, 512)])
+def test_more_choices_than_a_warp_has_lanes(t, k, d):
+    """A plan of ids chosen elsewhere has no limit on k, and may name an expert twice."""
+    torch.manual_seed(k)
+    ids = torch.randint(-1, 6, (t, k), dtype=torch.int32, device="cuda")
+    plan = fn.moe_plan(ids, 6)
+    y = torch.randn(t * k, d, device="cuda").bfloat16().requires_grad_()
+    w = torch.rand(t, k, device="cuda").requires_grad_()
+    out = fn.moe_combine(y, w, plan)
+    kept = (ids >= 0)
+    for a in range(0, t, 1000):  # in parts: the rows in 64 bits are large
+        rows = y.detach()[plan.slots[a: a + 1000].long()].double() * kept[a: a + 1000, :, None]
+        terms = rows * w.detach()[a: a + 1000, :, None].double()
+        want = terms.sum(1)
+        near(out[a: a + 1000], want, BF * want.abs() + 2 * (2 * k + 2) * F32 * terms.abs().sum(1))
+    (dw,) = torch.autograd.grad(out, w, torch.ones_like(out))
+    near(dw[-50:], (y.detach()[plan.slots[-50:].long()].double() * kept[-50:, :, None]).sum(2), (d + 8) * F32 * 6 * d)
+    check_device_errors()
+
+
+@gpu
+def test_long_weight_gradients_do_not_drift():
+    """One group of 30000 rows: the tensor cores' truncating additions alone would be 3e-5 off in
+    the 2-norm. Partial sums of 512 rows, each of 32 truncated additions of 16 products, bound
+    the drift by 32 steps of 2^-23 of a partial sum; their fp32 sum rounds 59 times."""
+    torch.manual_seed(0)
+    x = torch.randn(30000, 256, device="cuda").bfloat16()
+    dy = torch.randn(30000, 264, device="cuda").bfloat16()
+    dw = grouped_wgrad(dy, x, ragged([30000], "cuda"))[0].double()
+    want = dy.double().t() @ x.double()
+    assert ((dw - want).norm() / want.norm()).item() < (32 * 2 + 59) * F32
+
+
+@gpu
+def test_gradients_have_no_second_derivative():
+    x = torch.randn(6, 16, device="cuda").bfloat16().requires_grad_()
+    logits = torch.randn(6, 4, device="cuda").requires_grad_()
+    weights, _, plan = fn.moe_route(logits, 2)
+    w = torch.randn(4, 8, 16, device="cuda").bfloat16().requires_grad_()
+    out = fn.moe_combine(fn.grouped_linear(fn.moe_dispatch(x, plan), w, plan.offsets), weights, plan)
+    (dx,) = torch.autograd.grad(out.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dx.float().sum().backward()
+
+
+@gpu
+def test_launch_counter_counts_backward_kernels():
+    from resihp.ops import _ext
+
+    counter = _ext.launch_counter()
+    before = (counter.launches, counter.enabled)
+    counter.launches, counter.enabled = 0, True
+    try:
+        x = torch.randn(40, 64, device="cuda").bfloat16().requires_grad_()
+        plan = fn.moe_plan(make_ids(40, 4, 2, 1).cuda(), 4)          # 2 kernels
+        y = fn.dropout(fn.moe_dispatch(x, plan), 0.1, 1)             # 2
+        torch.autograd.grad(y, x, torch.ones_like(y))                # 2
+        assert counter.launches == 6
+        counter.enabled = False
+        fn.moe_dispatch(x, plan)
+        assert counter.launches == 6
+    finally:
+        counter.launches, counter.enabled = before
+
+
+@gpu
+def test_fp32_rows_take_the_torch_path_on_the_gpu():
+    """Places out of range are left out there too, without a device-side index error."""
+    plan = fn.MoePlan(torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda"),
+                      torch.tensor([[0, 99], [-5, 3]], dtype=torch.int32, device="cuda"))
+    x = torch.randn(2, 7, device="cuda")
+    rows = fn.moe_dispatch(x, plan)
+    assert torch.equal(rows[0], x[0]) and torch.equal(rows[3], x[1]) and not rows[1:3].any()
+    out = fn.moe_combine(torch.ones(4, 7, device="cuda"), torch.ones(2, 2, device="cuda"), plan)
+    assert torch.equal(out, torch.ones(2, 7, device="cuda"))  # each token's other choice has no place
+    w = torch.randn(2, 5, 7, device="cuda")
+    near(grouped_linear(rows, w, plan.offsets)[0], x[0].double() @ w[0].double().t(), 1e-5)
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_no_tokens_at_all():
+    x, wr, wgu, wd = _block(5)
+    grads = _grads(wr, wgu, wd)
+    none = x[:0].clone().requires_grad_()
+    out = fn.moe_swiglu(none, wr, wgu, wd, 2, residual=none, grads=grads)
+    assert out.shape == (0, 128)
+    out.sum().backward()
+    assert none.grad.shape == (0, 128) and not any(g.any() for g in grads)
+
+
+@gpu
+def test_padding_takes_no_rows():
+    """Tokens whose logits are all -inf get no expert's row, weight or gradient, only the residual."""
+    x, wr, wgu, wd = _block(6)
+    pad = torch.zeros(300, dtype=torch.bool, device="cuda")
+    pad[250:] = True
+    x = x.clone()
+    x[pad] = float("nan")  # what lies in padded rows does not matter
+    logits = torch.where(pad[:, None], torch.full((), NINF, device="cuda"), fn.linear(torch.nan_to_num(x), wr).float())
+    weights, ids, plan = fn.moe_route(logits, 2)
+    assert int(plan.offsets[-1]) == 500 and (ids[pad] == -1).all() and not weights[pad].any()
+    rows = fn.moe_dispatch(x, plan)
+    y = fn.grouped_linear(fn.swiglu(fn.grouped_linear(rows, wgu, plan.offsets)), wd, plan.offsets)
+    out = fn.moe_combine(y, weights, plan)
+    assert out.isfinite().all() and not out[pad].any()
+    dw = grouped_wgrad(y, rows, plan.offsets)
+    assert dw.isfinite().all()
+
+
+@gpu
+def test_captured_large_products_replay():
+    """Products of many tiles per CTA pair in a graph, replayed with other offsets."""
+    x, w, dy, _ = _grouped_case([1500, 2596], 0, 2056, 520, seed=8)
+    offsets = ragged([1500, 2596], "cuda")
+    acc = torch.zeros(w.shape, device="cuda")
+
+    def step():
+        return grouped_linear(x, w, offsets), grouped_dgrad(dy, w, offsets), grouped_wgrad(dy, x, offsets, out=acc, accumulate=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for sizes in ([4096, 0], [1, 4095], [777, 3000]):
+        offsets.copy_(ragged(sizes, "cuda"))
+        acc.zero_()
+        graph.replay()
+        got = [t.clone() for t in outs]
+        assert torch.equal(got[0], grouped_linear(x, w, offsets)) and torch.equal(got[1], grouped_dgrad(dy, w, offsets))
+        assert torch.equal(got[2], grouped_wgrad(dy, x, offsets))
+    check_device_errors()
+
+
+@gpu
+def test_two_streams_at_once():
+    """The same operators on two streams at the same time, on their own rows."""
+    cases = [_block(s, t=700) for s in (20, 21)]
+    want = [fn.moe_swiglu(x, wr, wgu, wd, 2) for x, wr, wgu, wd in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, (x, wr, wgu, wd) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(fn.moe_swiglu(x, wr, wgu, wd, 2))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
