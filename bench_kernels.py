@@ -11,6 +11,7 @@
     python bench_kernels.py fused_ar [tp]  # fused GEMM->AR (no sequence parallelism), same shape
     python bench_kernels.py fused_time  # CUDA-event time of the emulated fused kernels vs the GEMM alone
     python bench_kernels.py mem_time  # achieved GB/s of RMSNorm, RoPE, SwiGLU and AdamW
+    python bench_kernels.py sparse_time  # router, row movements, grouped products and dropout
 
 Each workload touches a few hundred MB (more than the 126 MB L2, far below the device)
 and launches every kernel a handful of times, so a capture of one or two launches ends
@@ -228,6 +229,51 @@ def mem_time() -> None:
     print(json.dumps(out))
 
 
+def sparse_time() -> None:
+    """The sparse-MLP operators and dropout at the 1.3B micro-batch (4096 tokens, d 2048, FFN
+    5504, eight experts, two choices): time of each kernel call, GB/s of its algorithmic bytes
+    and TF/s of its products. Three sets of rows are used in turn (more than L2 together)."""
+    import json
+
+    t, d, f, e, c = 4096, 2048, 5504, 8, 2
+    k = ops._ext.require()
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    w = torch.empty(e, 2 * f, d, **bf).normal_(std=0.02)
+    acc = torch.zeros(e, 2 * f, d, device="cuda")
+    sets = []
+    for _ in range(3):
+        x, rows, dy = torch.randn(t, d, **bf), torch.randn(t * c, d, **bf), torch.randn(t * c, 2 * f, **bf)
+        logits = torch.randn(t, e, **bf)
+        sets.append((x, rows, dy, logits, *k.moe_route(logits, c, True)))
+    act, weights, flop = t * d * 2, w.numel() * 2, 2.0 * t * c * d * 2 * f
+    wide = t * c * 2 * f * 2
+    cases = {
+        "route": (lambda b: k.moe_route(b[3], c, True), t * (e * 2 + c * 12), 0),
+        "dispatch": (lambda b: k.moe_scatter(b[0], b[6], b[7]), (1 + c) * act, 0),
+        "dispatch_bwd": (lambda b: k.moe_gather(b[1], None, b[6], b[7], None), (1 + c) * act, 0),
+        "combine_residual": (lambda b: k.moe_gather(b[1], b[4], b[6], b[7], b[0]), (2 + c) * act, 0),
+        "combine_bwd": (lambda b: k.moe_combine_bwd(b[0], b[1], b[4], b[6], b[7]), (1 + 2 * c) * act, 0),
+        "grouped_fwd": (lambda b: k.grouped_rows(b[1], w, False, b[6]), weights + c * act + wide, flop),
+        "grouped_dgrad": (lambda b: k.grouped_rows(b[2], w, True, b[6]), weights + c * act + wide, flop),
+        "grouped_wgrad_acc": (lambda b: k.grouped_wgrad(b[2], b[1], b[6], acc, True), 4 * weights + c * act + wide, flop),
+        "dropout_residual": (lambda b: k.dropout(b[0], b[1][:t], 6554, 1, 2, None, 0), 3 * act, 0),
+    }
+    out = []
+    for name, (call, nbytes, flops) in cases.items():
+        i = [0]
+
+        def rotate():
+            call(sets[i[0] % 3])
+            i[0] += 1
+
+        us = _time_us(rotate, it=30, warm=6)
+        row = {"kernel": name, "us": round(us, 2), "gbs": round(nbytes / us / 1e3, 1)}
+        if flops:
+            row["tflops"] = round(flops / us / 1e6, 1)
+        out.append(row)
+    print(json.dumps(out))
+
+
 def fused_time() -> None:
     """CUDA-event time of the fused TP kernels with the peers emulated by local buffers
     (the kernel's structure without NVLink latency) against this package's GEMM alone
@@ -264,7 +310,7 @@ def main(argv=None) -> None:
             fused_rs(tp, all_reduce=what == "fused_ar")
     else:
         {"gemm": gemm, "attn": attn, "dp": dp, "reshard": reshard, "gemm_time": gemm_time,
-         "attn_time": attn_time, "fused_time": fused_time, "mem_time": mem_time}[what]()
+         "attn_time": attn_time, "fused_time": fused_time, "mem_time": mem_time, "sparse_time": sparse_time}[what]()
     torch.cuda.synchronize()
     ops.check_device_errors()
     print("ok", what)

@@ -10,8 +10,8 @@
 // alignment rule), reads into the next group where the group ends inside it, and stores only
 // its own rows. Weights are 3-D maps, so a tile never reads into the next group's matrix:
 // what lies past a matrix's edge is zero, and a next group's infinity or NaN cannot leak in.
-// The weight gradient's reduction does end inside a tile: the rows of the last K block that
-// belong to the next group are overwritten with zeros in shared memory before its MMAs.
+// The weight gradient's reduction does end inside a tile: the rows of its last MMA step that
+// belong to the next group are overwritten with zeros in shared memory first.
 // Rows behind the last group give zeros, so the output is defined everywhere.
 //
 // Every CTA reads the offsets itself and walks the same tile list (prefix sums of tiles per
@@ -19,7 +19,11 @@
 // that decrease or pass the row count are clamped (and kErrBounds recorded): no value in
 // them can send an access out of range.
 //
-// Roles as in gemm.cu: warp 0 loads, warp 1 issues the MMAs, warps 2-5 run the epilogue.
+// Roles as in gemm.cu, on CTA pairs: warp 0 loads, the leader's warp 1 issues the MMAs, the
+// others run the epilogue. The loading and issuing warps walk their loops whole and one lane of
+// them issues: their counters, addresses and descriptors are then the same in all lanes, which
+// the instructions want, and a block of 256 x 256 x 64 is issued in less than the 512 cycles
+// its MMAs take (from inside a branch on the lane it took 1000: 1234 TF/s forward, then 1366).
 #include <algorithm>
 
 #include "common.cuh"
@@ -111,6 +115,11 @@ __device__ __forceinline__ int group_of(const Lists& l, int groups, int t, int f
 // rows cost (at 8 groups of about 1024 rows, 256-row M tiles would do 12 % more work), and a
 // handful of rows costs one narrow MMA per K step while the weights stream past. A group of
 // more than TN rows is cut into equal parts, not into full tiles and a rest.
+//
+// Many rows: bound by the tensor cores, and in long products by the power cap: 8192 rows of
+// eight groups, 2048 > 11008, take 270 us forward and 266 backward (1366 and 1390 TF/s of the
+// 1643 a library product reaches in a burst, 1397 sustained). Few rows: bound by reading the
+// weights: 16 rows, same weights, 58 us (6.2 TB/s of the 6.5 a copy reaches).
 
 constexpr int kBK = 64;
 
@@ -328,6 +337,8 @@ __global__ void __launch_bounds__(192, 1)
 // warps per CTA keep 128 columns of a row per thread. The finished tile leaves through shared
 // memory as bulk stores or bulk additions (whole 128-byte runs, clipped at the matrix's edges
 // by the map): each element is added to once per launch, so no order can change the sum.
+// 8192 rows of eight groups, 2048 x 11008: 345 us written, 388 added to what is there (721 MB
+// of fp32, of which the sums alone would take 110 us and 220; the MMAs 270).
 //
 // A group's last block holds rows of the next group where its length is no multiple of 64.
 // Steps of 16 rows past the end are not issued; rows past the end inside the last step are
@@ -336,7 +347,7 @@ __global__ void __launch_bounds__(192, 1)
 
 constexpr int kWChunk = 8;       // blocks per accumulator
 constexpr int kWStages = 5;
-constexpr int kWThreads = 352;   // producer, MMA, zeroing, eight epilogue warps
+constexpr int kWThreads = 384;   // dy producer, MMA, zeroing, eight epilogue warps, x producer
 struct WgradTile {
   static constexpr int kChunkBytes = 64 * kBK * 2;  // 64 columns of a block, MN-major
   static constexpr int kABytes = 2 * kChunkBytes;   // this CTA's 128 columns of dy, then of x
@@ -405,9 +416,14 @@ __global__ void __launch_bounds__(kWThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // the whole warp walks, one lane issues
-    const uint32_t issue = elect_one(), lead = cta == 0 ? issue : 0u;
+  if (warp == 0 || warp == 11) {
+    // Two producers, one per operand: a load costs its warp about 120 cycles, and four of them
+    // per block would pace the MMAs (512 cycles; 8192 rows, 2048 x 11008, eight groups, written:
+    // 370 us with one producer, 345 with two). The whole warp walks, one lane issues.
+    const bool second = warp == 11;
+    const uint32_t issue = elect_one(), lead = cta == 0 && !second ? issue : 0u, own = second ? 0u : issue;
+    const CUtensorMap* map = second ? &tma_x : &tma_dy;
+    const int part = second ? S::kABytes : 0;
     const uint32_t sbase = smem_u32(smem), fbase = smem_u32(full), fleader = mapa_shared(full, 0);
     const uint32_t cbase = smem_u32(cut), cown = mapa_shared(cut, cta);
     int s = 0;
@@ -419,22 +435,20 @@ __global__ void __launch_bounds__(kWThreads, 1)
       tile_coords(t - e * per_group, tiles_m, tiles_n, tm, tn);
       int r0 = __shfl_sync(0xFFFFFFFFu, l.row[e], 0);
       int left = __shfl_sync(0xFFFFFFFFu, l.row[e + 1], 0) - r0;
-      const int m0 = tm * 256 + int(cta) * 128, n0 = tn * 256 + int(cta) * 128;
+      const int c0 = (second ? tn : tm) * 256 + int(cta) * 128;
       for (; left > 0; left -= kBK, r0 += kBK) {
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait))) { ok = false; break; }
         uint32_t bar = fleader + s * 8;
         if (left < kBK && is_cut(left)) {
           mbar_arrive_if(lead, fbase + s * 8);
-          mbar_expect_tx_if(issue, cbase + s * 8, S::kStageBytes);
+          mbar_expect_tx_if(own, cbase + s * 8, S::kStageBytes);
           bar = cown + s * 8;
         } else {
           mbar_expect_tx_if(lead, fbase + s * 8, 2 * S::kStageBytes);  // both CTAs' halves
         }
-        const uint32_t sa = sbase + s * S::kStageBytes;
-        tma_load_2d_pair_if(issue, sa, &tma_dy, bar, m0, r0, g.err);
-        tma_load_2d_pair_if(issue, sa + S::kChunkBytes, &tma_dy, bar, m0 + 64, r0, g.err);
-        tma_load_2d_pair_if(issue, sa + 2 * S::kChunkBytes, &tma_x, bar, n0, r0, g.err);
-        tma_load_2d_pair_if(issue, sa + 3 * S::kChunkBytes, &tma_x, bar, n0 + 64, r0, g.err);
+        const uint32_t dst = sbase + s * S::kStageBytes + part;
+        tma_load_2d_pair_if(issue, dst, map, bar, c0, r0, g.err);
+        tma_load_2d_pair_if(issue, dst + S::kChunkBytes, map, bar, c0 + 64, r0, g.err);
         if (++s == kWStages) { s = 0; ph ^= 1; }
       }
     }

@@ -57,7 +57,7 @@ __device__ __forceinline__ int expert_of(const int* ids, int64_t i, int start, i
   return e >= 0 && e < experts ? int(e) : experts;
 }
 
-__global__ void __launch_bounds__(1024) plan_count_kernel(const int* __restrict__ ids, int64_t pairs,
+__global__ void __launch_bounds__(1024) moe_plan_count_kernel(const int* __restrict__ ids, int64_t pairs,
                                                           int64_t pairs_per_block, int start, int experts,
                                                           int* __restrict__ counts) {
   pdl_enter();
@@ -128,7 +128,7 @@ __device__ __forceinline__ void place_pairs(const int* ids, int64_t first, int64
   }
 }
 
-__global__ void __launch_bounds__(1024) plan_place_kernel(const int* __restrict__ ids, int64_t pairs,
+__global__ void __launch_bounds__(1024) moe_plan_place_kernel(const int* __restrict__ ids, int64_t pairs,
                                                           int64_t pairs_per_block, int start, int experts,
                                                           const int* __restrict__ counts,
                                                           int* __restrict__ offsets, int* __restrict__ slots) {
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(const int* __restrict_
 // warp-wide reductions took 14 us for 32768 rows of 64 experts, four choices; this takes 9).
 // Lane j % LPR keeps choice j. A grid of one block goes on to sort its pairs itself.
 template <typename T, int LPR, int VPT, int KMAX>
-__global__ void __launch_bounds__(512) route_kernel(const T* __restrict__ logits, int64_t ld, int tokens, int experts,
+__global__ void __launch_bounds__(512) moe_route_kernel(const T* __restrict__ logits, int64_t ld, int tokens, int experts,
                                                     int k, bool normalize, int rows_per_block,
                                                     float* __restrict__ weights, int* ids, int* __restrict__ counts,
                                                     int* __restrict__ offsets, int* __restrict__ slots) {
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(512) route_kernel(const T* __restrict__ logits
 // between lanes. The softmax over all experts needs no sums again: choice 0 is the largest
 // logit, so p_e = w_0 exp(l_e - l_{id_0}).
 template <typename T, int KMAX>
-__global__ void __launch_bounds__(256) route_bwd_kernel(const T* __restrict__ logits, int64_t ld,
+__global__ void __launch_bounds__(256) moe_route_bwd_kernel(const T* __restrict__ logits, int64_t ld,
                                                         const float* __restrict__ weights, const int* __restrict__ ids,
                                                         const float* __restrict__ dweights, T* __restrict__ dlogits,
                                                         int tokens, int experts, int k, bool normalize, int lpr) {
@@ -371,7 +371,7 @@ constexpr int kTogether = 4;
 // Threads of a block: ``lpr`` per row (blockDim.x / lpr rows), grid.y over the row's vectors, U
 // vectors per thread.
 template <int VEC, int U, int J>
-__global__ void __launch_bounds__(256) gather_kernel(MoveArgs a, int lpr) {
+__global__ void __launch_bounds__(256) moe_gather_kernel(MoveArgs a, int lpr) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(256) gather_kernel(MoveArgs a, int lpr) {
 // of two choices, width 2048, with residual: 11.4 us (5.9 TB/s) with U = J = 2; U = 4 12.5,
 // J = 4 16.5 (fewer warps), a thread per vector 13.1.
 template <int VEC, int U, int J>
-__global__ void __launch_bounds__(256) gather_warp_kernel(MoveArgs a) {
+__global__ void __launch_bounds__(256) moe_gather_warp_kernel(MoveArgs a) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(256) gather_warp_kernel(MoveArgs a) {
 
 // Copies of a token's row at its pairs' places; zeros where no expert takes the pair.
 template <int VEC, int U>
-__global__ void __launch_bounds__(256) scatter_kernel(MoveArgs a, int lpr) {
+__global__ void __launch_bounds__(256) moe_scatter_kernel(MoveArgs a, int lpr) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(256) scatter_kernel(MoveArgs a, int lpr) {
 // token with two choices at a time 20.7. The products are summed lane, warp, pair in a fixed
 // order.
 template <int VEC, int U>
-__global__ void __launch_bounds__(256) combine_bwd_kernel(MoveArgs a, int lpr) {
+__global__ void __launch_bounds__(256) moe_combine_bwd_kernel(MoveArgs a, int lpr) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
@@ -617,7 +617,7 @@ int place_bytes(int experts, int warps) { return (2 + warps) * (experts + 1) * i
 void launch_place(const int* ids, int64_t pairs, int64_t per_block, int blocks, int start, int experts,
                   const int* counts, int* offsets, int* slots, cudaStream_t st) {
   const int warps = place_warps(experts, 16);
-  RESIHP_CUDA_CHECK(launch_pdl(plan_place_kernel, blocks, 32 * warps, place_bytes(experts, warps), st, ids, pairs,
+  RESIHP_CUDA_CHECK(launch_pdl(moe_plan_place_kernel, blocks, 32 * warps, place_bytes(experts, warps), st, ids, pairs,
                                per_block, start, experts, counts, offsets, slots));
 }
 
@@ -638,7 +638,7 @@ struct RouteCall {
 template <typename T, int LPR, int VPT, int KMAX>
 void launch_route_as(const RouteCall& c, cudaStream_t st) {
   const int warps = place_warps(c.experts, 16);
-  RESIHP_CUDA_CHECK(launch_pdl(route_kernel<T, LPR, VPT, KMAX>, c.blocks, 32 * warps, place_bytes(c.experts, warps), st,
+  RESIHP_CUDA_CHECK(launch_pdl(moe_route_kernel<T, LPR, VPT, KMAX>, c.blocks, 32 * warps, place_bytes(c.experts, warps), st,
                                static_cast<const T*>(c.logits), c.ld, c.tokens, c.experts, c.k, c.normalize,
                                c.rows_per_block, c.weights, c.ids, c.counts, c.offsets, c.slots));
 }
@@ -676,7 +676,7 @@ void launch_route_bwd(const void* logits, int64_t ld, const float* weights, cons
                       void* dlogits, int tokens, int experts, int k, bool normalize, cudaStream_t st) {
   int lpr = 1;
   while (lpr < 32 && lpr * 8 < experts) lpr <<= 1;
-  auto kernel = k <= 4 ? route_bwd_kernel<T, 4> : k <= 8 ? route_bwd_kernel<T, 8> : route_bwd_kernel<T, kMoeMaxChoices>;
+  auto kernel = k <= 4 ? moe_route_bwd_kernel<T, 4> : k <= 8 ? moe_route_bwd_kernel<T, 8> : moe_route_bwd_kernel<T, kMoeMaxChoices>;
   RESIHP_CUDA_CHECK(launch_pdl(kernel, up(tokens, 256 / lpr), 256, 0, st, static_cast<const T*>(logits), ld, weights,
                                ids, dweights, static_cast<T*>(dlogits), tokens, experts, k, normalize, lpr));
 }
@@ -716,7 +716,7 @@ void moe_plan(const int* ids, int64_t pairs, int start, int experts, int* counts
   RESIHP_CHECK(pairs <= kMoeMaxPairs, "moe_plan: tokens * k passes ", kMoeMaxPairs);
   const int64_t per_block = std::max(1, up(pairs, plan_blocks(pairs, num_sms)));
   const int blocks = std::max(1, up(pairs, per_block));
-  RESIHP_CUDA_CHECK(launch_pdl(plan_count_kernel, blocks, 1024, (experts + 1) * int(sizeof(int)), st, ids, pairs,
+  RESIHP_CUDA_CHECK(launch_pdl(moe_plan_count_kernel, blocks, 1024, (experts + 1) * int(sizeof(int)), st, ids, pairs,
                                per_block, start, experts, counts));
   launch_place(ids, pairs, per_block, blocks, start, experts, counts, offsets, slots, st);
 }
@@ -726,8 +726,8 @@ void moe_scatter(const void* x, const int* slots, const int* used, void* out, in
   MoveArgs a{x, nullptr, nullptr, nullptr, out, nullptr, slots, used, tokens, k, d, err};
   check_move(a);
   if (tokens == 0) return;
-  if (vectors(a)) launch_rows<8, 1>(scatter_kernel<8, 1>, a, st);
-  else launch_rows<1, 4>(scatter_kernel<1, 4>, a, st);
+  if (vectors(a)) launch_rows<8, 1>(moe_scatter_kernel<8, 1>, a, st);
+  else launch_rows<1, 4>(moe_scatter_kernel<1, 4>, a, st);
 }
 
 void moe_gather(const void* y, const float* weights, const void* residual, const int* slots, const int* used, void* out,
@@ -737,11 +737,11 @@ void moe_gather(const void* y, const float* weights, const void* residual, const
   if (tokens == 0) return;
   const bool many = tokens >= num_sms * 16;
   if (!vectors(a)) {
-    launch_rows<1, 4>(gather_kernel<1, 4, kTogether>, a, st);
+    launch_rows<1, 4>(moe_gather_kernel<1, 4, kTogether>, a, st);
   } else if (many && d >= 256 && k <= 32) {  // (a lane of the warp holds a choice's place)
-    RESIHP_CUDA_CHECK(launch_pdl(gather_warp_kernel<8, 2, 2>, up(tokens, 8), 256, 0, st, a));
+    RESIHP_CUDA_CHECK(launch_pdl(moe_gather_warp_kernel<8, 2, 2>, up(tokens, 8), 256, 0, st, a));
   } else {
-    launch_rows<8, 1>(many ? gather_kernel<8, 1, 1> : gather_kernel<8, 1, kTogether>, a, st);
+    launch_rows<8, 1>(many ? moe_gather_kernel<8, 1, 1> : moe_gather_kernel<8, 1, kTogether>, a, st);
   }
 }
 
@@ -754,7 +754,7 @@ void moe_combine_bwd(const void* dout, const void* y, const float* weights, cons
   const int vpr = vec ? d / 8 : d;
   const int lpr = int64_t(tokens) * k >= int64_t(num_sms) * 16 ? 32 : std::max(32, lanes_for(vpr));
   const int grid = up(int64_t(tokens) * k, 256 / lpr);
-  auto kernel = vec ? (vpr <= lpr ? combine_bwd_kernel<8, 1> : combine_bwd_kernel<8, 4>) : combine_bwd_kernel<1, 4>;
+  auto kernel = vec ? (vpr <= lpr ? moe_combine_bwd_kernel<8, 1> : moe_combine_bwd_kernel<8, 4>) : moe_combine_bwd_kernel<1, 4>;
   RESIHP_CUDA_CHECK(launch_pdl(kernel, grid, 256, 0, st, a, lpr));
 }
 

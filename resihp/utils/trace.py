@@ -57,6 +57,9 @@ _CATEGORIES = (
     (r"gemm_kernel<\d+, true, true|gemm_kernelILi\d+ELb1ELb1E"
      r"|gemm_pair_kernel<true, true|gemm_pair_kernelILb1ELb1E", "GEMM wgrad"),
     (r"gemm_(pair_)?kernel", "GEMM other"),
+    (r"grouped_(rows|wgrad)_kernel", "products grouped by expert"),
+    (r"moe_\w+_kernel", "sparse MLP routing"),
+    (r"dropout(_any)?_kernel", "dropout"),
     (r"attn_fwd_kernel", "attention forward"),
     (r"attn_bwd|attn_delta", "attention backward"),
     (r"rmsnorm|column_sum", "RMSNorm"),
