@@ -40,6 +40,7 @@ struct Args {
   int64_t ldc;
   const int* offsets;
   int groups, rows, n, k;
+  unsigned* pace;  // rows: see pace_pairs; nullptr: pairs run freely
   int* err;
 };
 
@@ -153,6 +154,31 @@ __device__ __forceinline__ RowSpan span_of(const Lists& l, int e, int t, int til
   return RowSpan{l.row[e] + tm * each, min(each, size - tm * each), tf * 256};
 }
 
+// Pacing. The tiles under way at one time share operand tiles: 74 pairs read about 17 panels of
+// 256 rows or features at once. Pairs that drift apart by more than L2 holds of those read the
+// same bytes again from memory: 16384 rows, 13824 > 5120, eight uneven groups, brought 7.7 GB
+// in where 1.6 are needed, and the last pair ended 18 % after the first. Where the panels of a
+// round pass half of L2 (k from 7168 on) every pair therefore counts itself in each 64 K
+// blocks, and waits a moment while another is two such steps behind: 1122 -> 1220 TF/s
+// there under the power cap; at k = 5504 and 11008 (8192 rows) it neither gains nor costs.
+constexpr int kPaceBlocks = 64;
+constexpr int kPaceDepth = 7168;
+constexpr uint64_t kPaceNs = 20000;
+
+// One lane of every pair, at each step. False once the others take too long (pairs that are not
+// resident, a device that is shared): the pair then runs freely, as nothing but time depends on
+// it.
+__device__ __forceinline__ bool pace_pairs(unsigned* count, unsigned step, unsigned pairs) {
+  atomicAdd(count, 1u);
+  if (step == 0) return true;
+  const uint64_t start = globaltimer();
+  while (*reinterpret_cast<volatile unsigned*>(count) < step * pairs) {
+    if (globaltimer() - start > kPaceNs) return false;
+    __nanosleep(64);
+  }
+  return true;
+}
+
 template <int TN, bool W_MN>
 __global__ void __launch_bounds__(192, 1)
     grouped_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_a, Args g) {
@@ -207,7 +233,10 @@ __global__ void __launch_bounds__(192, 1)
     int s = 0, e = 0;
     uint32_t ph = 0;
     bool ok = true;
+    bool paced = g.pace != nullptr;  // the same in all lanes
+    unsigned step = 0;
     for (int t = pair; t < work && ok; t += pairs) {
+      paced = paced && t - pair + pairs <= work;  // not in the last round, which some pairs sit out
       e = group_of(l, g.groups, t, e);
       const RowSpan p = span_of<TN>(l, e, t, tiles_f);
       // each CTA brings its features and its half of the MMA's N rows
@@ -215,6 +244,12 @@ __global__ void __launch_bounds__(192, 1)
       const int r0 = __shfl_sync(0xFFFFFFFFu, p.row0 + int(cta) * (mma_rows(p.rows) >> 1), 0);
       const int plane = __shfl_sync(0xFFFFFFFFu, e, 0);
       for (int kb = 0; kb < kblocks; ++kb) {
+        if (paced && kb % kPaceBlocks == 0) {
+          bool in_time = true;
+          if (lead) in_time = pace_pairs(g.pace, step, unsigned(pairs));
+          paced = __all_sync(0xFFFFFFFFu, in_time);
+          ++step;
+        }
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(&empty[s], ph ^ 1, g.err, kErrTmaWait))) { ok = false; break; }
         const uint32_t sw = sbase + s * S::kStageBytes, bar = fleader + s * 8;
         mbar_expect_tx_if(lead, fbase + s * 8, 2 * S::kStageBytes);  // both CTAs' parts
@@ -695,12 +730,17 @@ void check_shape(const GroupedShape& s) {
 
 }  // namespace
 
+bool grouped_paces(const GroupedShape& s) {
+  return s.k >= kPaceDepth && int64_t(s.rows / 256) * ((s.n + 255) / 256) >= num_sms();
+}
+
 void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t w_group, bool w_mn, void* c,
-                  int64_t ldc, const GroupedShape& s, int* err, cudaStream_t st) {
+                  int64_t ldc, const GroupedShape& s, unsigned* pace, int* err, cudaStream_t st) {
   check_shape(s);
   if (s.rows == 0) return;
+  if (pace != nullptr) RESIHP_CUDA_CHECK(cudaMemsetAsync(pace, 0, sizeof(unsigned), st));
   RESIHP_CHECK(reinterpret_cast<uintptr_t>(c) % 16 == 0 && ldc % 8 == 0, "grouped output must be 16-byte aligned");
-  const Args g{c, ldc, s.offsets, s.groups, s.rows, s.n, s.k, err};
+  const Args g{c, ldc, s.offsets, s.groups, s.rows, s.n, s.k, pace, err};
   // Few rows per group: the weights' bytes set the time, and narrow row tiles leave room for
   // eight of their stages in flight instead of six. At 100 rows a group (eight groups, 2048 >
   // 11008) 64.3 against 66.7 us, at 94 uneven ones (64 groups, 1024 > 1416) 44.3 against 46.9;
@@ -722,7 +762,7 @@ void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, flo
   const CUtensorMap tdy = make_tma_2d_bf16(dy, s.rows, s.n, lddy, 64, kBK);
   const CUtensorMap tx = make_tma_2d_bf16(x, s.rows, s.k, ldx, 64, kBK);
   const CUtensorMap tc = make_tma_3d_f32(c, s.groups, s.n, s.k, 32);
-  const Args g{c, 0, s.offsets, s.groups, s.rows, s.n, s.k, err};
+  const Args g{c, 0, s.offsets, s.groups, s.rows, s.n, s.k, nullptr, err};
   if (accumulate) launch_wgrad<true>(tiles, tdy, tx, tc, g, st);
   else launch_wgrad<false>(tiles, tdy, tx, tc, g, st);
 }

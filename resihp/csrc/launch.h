@@ -212,9 +212,12 @@ struct GroupedShape {
   int groups, rows;    // rows: of the row operands; those behind the last group's give zeros
   int n, k;            // output columns, reduction length (wgrad: output rows x columns)
 };
-// c[r, n] = sum_k a[r, k] w[g(r), n, k] (w_mn: w[g(r), k, n]), bf16.
+// c[r, n] = sum_k a[r, k] w[g(r), n, k] (w_mn: w[g(r), k, n]), bf16. pace: one word of device
+// memory for this call alone where grouped_paces says so (its CTAs keep step through it),
+// nullptr otherwise.
+bool grouped_paces(const GroupedShape& s);
 void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t w_group, bool w_mn, void* c,
-                  int64_t ldc, const GroupedShape& s, int* err, cudaStream_t st);
+                  int64_t ldc, const GroupedShape& s, unsigned* pace, int* err, cudaStream_t st);
 // c[g, n, k] (+)= sum over the group's rows of dy[r, n] x[r, k], fp32 [groups, n, k] contiguous.
 void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, float* c, bool accumulate,
                    const GroupedShape& s, int* err, cudaStream_t st);

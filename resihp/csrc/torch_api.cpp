@@ -459,8 +459,11 @@ torch::Tensor grouped_rows_t(torch::Tensor a, torch::Tensor w, bool w_mn, torch:
   const GroupedShape s = grouped_shape(a, offsets, n, k);
   c10::cuda::CUDAGuard guard(a.device());
   auto c = torch::empty({a.size(0), n}, a.options());
+  torch::Tensor pace;  // this call's own: calls on other streams and in graphs have theirs
+  if (grouped_paces(s)) pace = torch::empty({1}, offsets.options());
   grouped_rows(a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(1), w.stride(0), w_mn, c.data_ptr(), n, s,
-               error_word(a.device()), cur_stream());
+               pace.defined() ? reinterpret_cast<unsigned*>(pace.data_ptr<int>()) : nullptr, error_word(a.device()),
+               cur_stream());
   count_launches(s.rows > 0);
   return c;
 }

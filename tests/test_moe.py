@@ -911,3 +911,33 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+@gpu
+def test_paced_products_in_graphs_and_on_two_streams():
+    """Products deep and large enough that their CTA pairs keep step: alone, two at once (not all
+    pairs resident) and replayed from a graph they give the same rows."""
+    rows, n, k = 4200, 2568, 7176
+    x, w, dy, offsets = _grouped_case([3000, 1100], 100, n, k, seed=9)
+    y = grouped_linear(x, w, offsets)
+    for g, at in ((0, slice(0, 300)), (0, slice(2900, 3000)), (1, slice(3000, 3100)), (1, slice(4000, 4100))):
+        want, size = x[at].double() @ w[g].double().t(), x[at].double().abs() @ w[g].double().abs().t()
+        near(y[at], want, BF * want.abs() + 1.01 * 2 * k * F32 * size)
+    assert not y[4100:].any()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(grouped_linear(x, w, offsets))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, y) for o in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = grouped_linear(x, w, offsets)
+    for sizes in ([3000, 1100], [17, 4183], [0, 4200]):
+        offsets.copy_(ragged(sizes, "cuda"))
+        graph.replay()
+        assert torch.equal(out, grouped_linear(x, w, offsets))
+    check_device_errors()
