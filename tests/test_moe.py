@@ -941,3 +941,35 @@ def test_paced_products_in_graphs_and_on_two_streams():
         graph.replay()
         assert torch.equal(out, grouped_linear(x, w, offsets))
     check_device_errors()
+
+
+@gpu
+def test_grouped_gradient_of_a_sum():
+    """The gradient arrives as one value with stride 0, and goes to a view of a larger leaf."""
+    big = torch.randn(60, 2, 64, device="cuda").bfloat16().requires_grad_()
+    w = torch.randn(2, 40, 64, device="cuda").bfloat16()
+    offsets = ragged([25, 35], "cuda")
+    fn.grouped_linear(big[:, 1], w, offsets).sum().backward()
+    own = owners([25, 35], 60).cuda()
+    want = w.double().sum(1)[own]
+    near(big.grad[:, 1], want, BF * want.abs() + 2 * 40 * F32 * w.double().abs().sum(1)[own])
+    assert not big.grad[:, 0].any()
+
+
+@gpu
+def test_recomputed_block_gives_the_same_gradients():
+    from torch.utils.checkpoint import checkpoint
+
+    x, wr, wgu, wd = _block(7)
+    results = []
+    for recompute in (False, True):
+        grads, leaf = _grads(wr, wgu, wd), x.clone().requires_grad_()
+        wr.requires_grad_(), wgu.requires_grad_(), wd.requires_grad_()
+
+        def layer(t):
+            return fn.dropout(fn.moe_swiglu(t, wr, wgu, wd, 2, grads=grads), 0.1, 3, 4, residual=t)
+
+        out = checkpoint(layer, leaf, use_reentrant=False) if recompute else layer(leaf)
+        out.backward(torch.ones_like(out))
+        results.append((out.detach(), leaf.grad, *grads))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
