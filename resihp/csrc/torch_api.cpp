@@ -8,9 +8,11 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <atomic>
+#include <unordered_set>
 #include <mutex>
 #include <csignal>
 #include <execinfo.h>
@@ -493,6 +495,31 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = c10::optional<torch::Tensor>;
 
+// First in every backward pass. A leaf keeps the stream its first living graph was recorded on,
+// and the engine joins that stream with the pass's, with or without a gradient for the leaf. If
+// it is the default stream and the pass is being captured, the join is not allowed and the
+// process may end in the engine, so it is refused here, where it is still an error, for every
+// leaf that the pass will reach from here.
+static void check_capture() {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto current = torch::autograd::get_current_node();
+  std::vector<torch::autograd::Node*> todo = {current.get()};
+  std::unordered_set<torch::autograd::Node*> seen = {current.get()};
+  while (!todo.empty()) {
+    torch::autograd::Node* node = todo.back();
+    todo.pop_back();
+    if (node == nullptr) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node) != nullptr) {
+      const auto stream = node->stream();
+      TORCH_CHECK(!stream.has_value() || stream->id() != 0,
+                  "a backward pass cannot be captured while a graph of the same leaf recorded on the default stream "
+                  "is alive: drop its outputs, or record it on another stream");
+    }
+    for (size_t i = 0; i < node->num_outputs(); ++i)
+      if (node->task_should_compute_output(i) && seen.insert(node->next_edge(i).function.get()).second)
+        todo.push_back(node->next_edge(i).function.get());
+  }
+}
 
 // These gradients have no derivative of their own: asking for one raises.
 static variable_list once(variable_list grads) {
@@ -514,6 +541,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     return dropout_t(x.contiguous(), rows_of(residual), drop, seed, offset, state, first);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     const auto a = ctx->saved_data["args"].toIntVector();
     OptTensor state;
     if (a[5]) state = ctx->get_saved_variables()[0];
@@ -534,6 +562,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     if (!grads[0].defined()) return {{}, {}, {}};
     const auto saved = ctx->get_saved_variables();
     return once({moe_route_bwd_t(saved[0], saved[1], saved[2], grads[0].contiguous(),
@@ -548,6 +577,7 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
     return moe_scatter_t(x.contiguous(), offsets, slots);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     const auto saved = ctx->get_saved_variables();
     return once({moe_gather_t(grads[0].contiguous(), c10::nullopt, saved[0], saved[1], c10::nullopt), {}, {}});
   }
@@ -563,6 +593,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     return moe_gather_t(rows, w, offsets, slots, rows_of(residual));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     const auto saved = ctx->get_saved_variables();
     std::vector<torch::Tensor> d(2);
     if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1))
@@ -588,6 +619,7 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     return grouped_rows_t(xt, wt, false, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     const auto saved = ctx->get_saved_variables();
     const auto dy = tiles_of(grads[0]);
     torch::Tensor dx, dw;

@@ -973,3 +973,68 @@ def test_recomputed_block_gives_the_same_gradients():
         out.backward(torch.ones_like(out))
         results.append((out.detach(), leaf.grad, *grads))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@gpu
+@pytest.mark.parametrize("op", ["dropout", "route", "dispatch", "combine", "residual", "grouped", "behind"])
+def test_capture_beside_an_eager_graph_is_refused(op):
+    """While a graph of the same leaf, recorded on the default stream, is alive, a captured backward
+    pass raises; without it the pass is captured and replays."""
+    x = torch.randn(64, 64, device="cuda").bfloat16().requires_grad_()
+    w = torch.randn(2, 16, 64, device="cuda").bfloat16()
+    _, ids, plan = fn.moe_route(torch.randn(64, 2, device="cuda"), 1)
+    weights = torch.rand(64, 1, device="cuda")
+    rows = torch.randn(64, 64, device="cuda").bfloat16()
+    call = {
+        "dropout": lambda: fn.dropout(x, 0.25, 3),
+        "route": lambda: fn.moe_route(x, 2)[0],
+        "dispatch": lambda: fn.moe_dispatch(x, plan),
+        "combine": lambda: fn.moe_combine(x, weights, plan),
+        "residual": lambda: fn.moe_combine(rows, weights, plan, residual=x),
+        "grouped": lambda: fn.grouped_linear(x, w, plan.offsets),
+        "behind": lambda: fn.dropout(x.view(32, 128) * 2, 0.25, 3),
+    }[op]
+
+    def step():
+        out = call()
+        return torch.autograd.grad(out, x, out.detach())[0]
+
+    want = step()
+    alive = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+        with pytest.raises(RuntimeError, match="default stream"):
+            torch.autograd.grad(out, x, out.detach())
+    del alive, out, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    assert torch.equal(got, want)
+    check_device_errors()
+
+
+@gpu
+def test_capture_past_a_leaf_of_an_eager_graph():
+    """Weights in a living eager graph: a captured pass that asks for the rows' gradient alone does
+    not reach them and is captured, main gradient included; one that reaches them raises."""
+    x = torch.randn(64, 64, device="cuda").bfloat16()
+    w = torch.randn(2, 16, 64, device="cuda").bfloat16().requires_grad_()
+    offsets = ragged([40, 24], "cuda")
+    acc = torch.zeros(2, 16, 64, device="cuda")
+    alive = fn.grouped_linear(x, w, offsets, main_grad=acc)
+    alive.backward(alive.detach(), retain_graph=True)
+    want = acc.clone()
+    leaf = x.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fn.grouped_linear(leaf, w, offsets, main_grad=acc)
+        (dx,) = torch.autograd.grad(out, leaf, out.detach(), retain_graph=True)
+        with pytest.raises(RuntimeError, match="default stream"):
+            out.backward(out.detach())
+    acc.zero_()
+    graph.replay()
+    assert torch.equal(acc, want) and torch.equal(dx, grouped_dgrad(alive.detach(), w, offsets))
+    assert w.grad is None and leaf.grad is None
+    check_device_errors()
