@@ -415,7 +415,7 @@ __device__ __forceinline__ void wgrad_coords(int t, int blocks, int tiles_m, int
 __device__ __forceinline__ int valid_rows(int size, int kb) { return min(kBK, size - kb * kBK); }
 __device__ __forceinline__ bool is_cut(int valid) { return (valid & 15) != 0; }
 
-template <bool ACC>
+template <bool ACC, bool BF16>
 __global__ void __launch_bounds__(kWThreads, 1)
     grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tma_dy, const __grid_constant__ CUtensorMap tma_x,
                          const __grid_constant__ CUtensorMap tma_c, Args g) {
@@ -636,20 +636,29 @@ __global__ void __launch_bounds__(kWThreads, 1)
       wgrad_coords(t - e * per_group, blocks, tiles_m, tiles_n, tm, tn);
       const int row0 = tm * 256 + int(cta) * 128 + q * 32, col0 = tn * 256 + half * 128;
       if (row0 >= g.n) continue;
+      constexpr int kCols = BF16 ? 64 : 32;  // of a 128-byte row of staging
       #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // 32 columns at a time
-        if (col0 + j * 32 < g.k) {
+      for (int j = 0; j < 128; j += kCols) {
+        if (col0 + j < g.k) {
           if (lane == 0) bulk_wait_read_all();
           __syncwarp();
           #pragma unroll
-          for (int x = 0; x < 8; ++x)  // the map's 128-byte swizzle: 16-byte unit x of row r is at x ^ r % 8
-            *reinterpret_cast<float4*>(buf + lane * 128 + ((x ^ (lane & 7)) << 4)) =
-                make_float4(acc[j * 32 + 4 * x], acc[j * 32 + 4 * x + 1], acc[j * 32 + 4 * x + 2], acc[j * 32 + 4 * x + 3]);
+          for (int x = 0; x < 8; ++x) {  // the map's 128-byte swizzle: 16-byte unit x of row r is at x ^ r % 8
+            uint8_t* unit = buf + lane * 128 + ((x ^ (lane & 7)) << 4);
+            if (BF16) {
+              const float* v = acc + j + 8 * x;  // the one rounding of the sum
+              *reinterpret_cast<uint4*>(unit) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
+                                                           pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+            } else {
+              const float* v = acc + j + 4 * x;
+              *reinterpret_cast<float4*>(unit) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+          }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            if (ACC) tma_add_3d_f32(&tma_c, buf, col0 + j * 32, row0, e, g.err);
-            else tma_store_3d_f32(&tma_c, buf, col0 + j * 32, row0, e, g.err);
+            if (ACC) tma_add_3d_f32(&tma_c, buf, col0 + j, row0, e, g.err);
+            else tma_store_3d(&tma_c, buf, col0 + j, row0, e, g.err);
             bulk_commit();
           }
         }
@@ -717,11 +726,11 @@ void launch_rows(int64_t tiles, const CUtensorMap& tw, const CUtensorMap& ta, co
   launch_pairs(grouped_rows_kernel<TN, W_MN>, resident, 192, RowTile<TN>::kSmem, tiles, st, tw, ta, g);
 }
 
-template <bool ACC>
+template <bool ACC, bool BF16>
 void launch_wgrad(int64_t tiles, const CUtensorMap& tdy, const CUtensorMap& tx, const CUtensorMap& tc, const Args& g,
                   cudaStream_t st) {
   static int resident[64] = {0};
-  launch_pairs(grouped_wgrad_kernel<ACC>, resident, kWThreads, WgradTile::kSmem, tiles, st, tdy, tx, tc, g);
+  launch_pairs(grouped_wgrad_kernel<ACC, BF16>, resident, kWThreads, WgradTile::kSmem, tiles, st, tdy, tx, tc, g);
 }
 
 template <int TN>
@@ -765,22 +774,25 @@ void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_
   else launch_rows_tn<256>(a, lda, w, ldw, w_group, w_mn, s, g, st);
 }
 
-void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, float* c, bool accumulate,
+void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c, bool bf16, bool accumulate,
                    const GroupedShape& s, int* err, cudaStream_t st) {
   check_shape(s);
   RESIHP_CHECK(reinterpret_cast<uintptr_t>(c) % 16 == 0, "grouped weight gradient must be 16-byte aligned");
+  RESIHP_CHECK(!bf16 || !accumulate, "grouped weight gradient: only fp32 is accumulated into");
   if (s.rows == 0) {
-    if (!accumulate) RESIHP_CUDA_CHECK(cudaMemsetAsync(c, 0, sizeof(float) * size_t(s.groups) * s.n * s.k, st));
+    if (!accumulate) RESIHP_CUDA_CHECK(cudaMemsetAsync(c, 0, (bf16 ? 2 : 4) * size_t(s.groups) * s.n * s.k, st));
     return;
   }
   const int64_t tiles = int64_t(s.groups) * ((s.n + 255) / 256) * ((s.k + 255) / 256);
   RESIHP_CHECK(tiles <= INT32_MAX, "grouped products: too many tiles");
   const CUtensorMap tdy = make_tma_2d_bf16(dy, s.rows, s.n, lddy, 64, kBK);
   const CUtensorMap tx = make_tma_2d_bf16(x, s.rows, s.k, ldx, 64, kBK);
-  const CUtensorMap tc = make_tma_3d_f32(c, s.groups, s.n, s.k, 32);
+  const CUtensorMap tc = bf16 ? make_tma_3d_bf16(c, s.groups, s.n, s.k, s.k, int64_t(s.n) * s.k, 64, 32)
+                              : make_tma_3d_f32(c, s.groups, s.n, s.k, 32);
   const Args g{c, 0, s.offsets, s.groups, s.rows, s.n, s.k, nullptr, err};
-  if (accumulate) launch_wgrad<true>(tiles, tdy, tx, tc, g, st);
-  else launch_wgrad<false>(tiles, tdy, tx, tc, g, st);
+  if (accumulate) launch_wgrad<true, false>(tiles, tdy, tx, tc, g, st);
+  else if (bf16) launch_wgrad<false, true>(tiles, tdy, tx, tc, g, st);
+  else launch_wgrad<false, false>(tiles, tdy, tx, tc, g, st);
 }
 
 }  // namespace resihp

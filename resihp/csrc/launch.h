@@ -218,8 +218,9 @@ struct GroupedShape {
 bool grouped_paces(const GroupedShape& s);
 void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t w_group, bool w_mn, void* c,
                   int64_t ldc, const GroupedShape& s, unsigned* pace, int* err, cudaStream_t st);
-// c[g, n, k] (+)= sum over the group's rows of dy[r, n] x[r, k], fp32 [groups, n, k] contiguous.
-void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, float* c, bool accumulate,
+// c[g, n, k] (+)= sum over the group's rows of dy[r, n] x[r, k], [groups, n, k] contiguous, fp32 or
+// (written only) bf16.
+void grouped_wgrad(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c, bool bf16, bool accumulate,
                    const GroupedShape& s, int* err, cudaStream_t st);
 CUtensorMap make_tma_3d_bf16(const void* base, int64_t planes, int64_t rows, int64_t cols, int64_t ld, int64_t plane_ld,
                              int box_cols, int box_rows);

@@ -476,11 +476,13 @@ void grouped_wgrad_t(torch::Tensor dy, torch::Tensor x, torch::Tensor offsets, t
   TORCH_CHECK(dy.dim() == 2 && x.dim() == 2 && dy.stride(1) == 1 && x.stride(1) == 1 && dy.size(0) == x.size(0) &&
                   dy.device() == x.device(), "grouped wgrad needs dy [rows, N] and x [rows, K]");
   const GroupedShape s = grouped_shape(dy, offsets, dy.size(1), x.size(1));
-  TORCH_CHECK(out.device() == dy.device() && out.scalar_type() == at::kFloat && out.is_contiguous() && out.dim() == 3 &&
-                  out.size(0) == s.groups && out.size(1) == s.n && out.size(2) == s.k,
-              "grouped weight gradient must be contiguous fp32 [groups, N, K]");
+  const bool bf16 = out.scalar_type() == at::kBFloat16;
+  TORCH_CHECK(out.device() == dy.device() && (out.scalar_type() == at::kFloat || (bf16 && !accumulate)) &&
+                  out.is_contiguous() && out.dim() == 3 && out.size(0) == s.groups && out.size(1) == s.n &&
+                  out.size(2) == s.k,
+              "grouped weight gradient must be contiguous [groups, N, K], fp32 or, written, bf16");
   c10::cuda::CUDAGuard guard(dy.device());
-  grouped_wgrad(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), out.data_ptr<float>(), accumulate, s,
+  grouped_wgrad(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), out.data_ptr(), bf16, accumulate, s,
                 error_word(dy.device()), cur_stream());
   count_launches(s.rows > 0);
 }
@@ -628,9 +630,8 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     if (acc != ctx->saved_data.end()) {
       grouped_wgrad_t(dy, saved[0], saved[2], acc->second.toTensor(), true);
     } else if (ctx->needs_input_grad(1)) {
-      auto sum = torch::empty(saved[1].sizes(), saved[1].options().dtype(torch::kFloat));
-      grouped_wgrad_t(dy, saved[0], saved[2], sum, false);
-      dw = sum.to(saved[1].scalar_type());
+      dw = torch::empty(saved[1].sizes(), saved[1].options());
+      grouped_wgrad_t(dy, saved[0], saved[2], dw, false);
     }
     return once({dx, dw, {}, {}});
   }

@@ -1038,3 +1038,18 @@ def test_capture_past_a_leaf_of_an_eager_graph():
     assert torch.equal(acc, want) and torch.equal(dx, grouped_dgrad(alive.detach(), w, offsets))
     assert w.grad is None and leaf.grad is None
     check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("sizes, n, k", [([3, 0, 70], 40, 72), ([600, 1, 1500], 264, 328), ([0, 0], 16, 8),
+                                         ([130] * 9, 512, 1096), ([], 8, 8)])
+def test_grouped_weight_gradient_in_the_weights_type(sizes, n, k):
+    """Without a main gradient the weights' bf16 gradient is the fp32 sum rounded once, everywhere
+    (groups without rows get zeros)."""
+    x, w, dy, _ = _grouped_case(sizes or [0], 3, n, k, seed=5)
+    offsets = ragged(sizes or [0], "cuda")
+    w.requires_grad_()
+    fn.grouped_linear(x, w, offsets).backward(dy)
+    assert w.grad.dtype == torch.bfloat16
+    assert torch.equal(w.grad, grouped_wgrad(dy, x, offsets).bfloat16())
+    check_device_errors()
