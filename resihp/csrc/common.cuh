@@ -398,6 +398,13 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same arrival, relaxed: for a barrier that hands over tensor memory alone. The thread's
+// tcgen05.ld are complete (tcgen05.wait::ld) and ordered before it by tc_fence_before; a release
+// would in addition wait for its outstanding stores, of which the waiter reads none.
+__device__ __forceinline__ void mbar_arrive_remote_tmem(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // mbar_wait with acquire at cluster scope, for a barrier that CTAs of the cluster arrive on.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err, int code) {
   const uint32_t b = smem_u32(bar);

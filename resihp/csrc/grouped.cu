@@ -373,7 +373,8 @@ __global__ void __launch_bounds__(192, 1)
 // memory as bulk stores or bulk additions (whole 128-byte runs, clipped at the matrix's edges
 // by the map): each element is added to once per launch, so no order can change the sum.
 // 8192 rows of eight groups, 2048 x 11008: 345 us written, 388 added to what is there (721 MB
-// of fp32, of which the sums alone would take 110 us and 220; the MMAs 270).
+// of fp32, of which the sums alone would take 110 us and 220; the MMAs 270). As a bf16 gradient,
+// rounded once from the fp32 sum, 265 us; written in fp32 and cast by another kernel 440.
 //
 // A group's last block holds rows of the next group where its length is no multiple of 64.
 // Steps of 16 rows past the end are not issued; rows past the end inside the last step are
@@ -627,9 +628,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
           #pragma unroll
           for (int x = 0; x < 16; ++x) acc[j * 16 + x] += __uint_as_float(v[x]);
         }
+        // Relaxed: this lane's bulk stores of the last tile are still under way, and a release
+        // waits for them (1500 to 2400 cycles per tile; 64 groups of 94 rows, 1024 x 1416, written
+        // 83 us against 93). In the row products, whose stores are smaller, it made no difference.
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(a == 0 ? acc_empty_leader0 : acc_empty_leader1);
+        if (lane == 0) mbar_arrive_remote_tmem(a == 0 ? acc_empty_leader0 : acc_empty_leader1);
       }
       if (!ok) break;
       int tm, tn;
