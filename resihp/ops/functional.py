@@ -59,13 +59,17 @@ class _Linear(Function):
         x, w = ctx.saved_tensors
         dy = dy.contiguous()
         dx = linear_dgrad(dy, w) if ctx.needs_input_grad[0] else None
+        dw = None
         if ctx.main_grad is not None:
             linear_wgrad(dy, x, out=ctx.main_grad, accumulate=True)
-        return dx, None, None, (dy if ctx.has_residual else None)
+        elif ctx.needs_input_grad[1]:
+            dw = linear_wgrad(dy, x).to(w.dtype)  # the one rounding of the fp32 sum
+        return dx, dw, None, (dy if ctx.has_residual else None)
 
 
 def linear(x, w, main_grad=None, residual=None):
-    """``x @ w.T`` (+ residual). CUDA: tcgen05 GEMM, wgrad accumulated into ``main_grad``."""
+    """``x @ w.T`` (+ residual). CUDA: tcgen05 GEMM, wgrad accumulated into ``main_grad`` where one
+    is given, and ``w``'s gradient otherwise."""
     if not on_kernels(x):
         y = F.linear(x, w)
         return y if residual is None else y + residual
@@ -232,8 +236,9 @@ def moe_swiglu(x, w_router, w_gate_up, w_down, k, *, normalize=True, residual=No
     ``w_router [E, d]`` gives the router logits (FP32 sums of ``x``'s products, rounded to its
     dtype), ``w_gate_up [E, 2F, d]`` and ``w_down [E, d, F]`` are the experts' fused gate / up
     and down projections. ``grads``: the FP32 main-grad buffers of the three weights in that
-    order (CUDA bf16; see :func:`linear`). On the kernels the router takes a multiple of 8
-    experts (its logits are a GEMM's output). The steps are :mod:`resihp.ops.moe`'s.
+    order (CUDA bf16; see :func:`linear`); a weight without one gets its gradient from
+    autograd. On the kernels the router takes a multiple of 8 experts (its logits are a GEMM's
+    output). The steps are :mod:`resihp.ops.moe`'s.
     """
     if not x.shape[0]:
         return torch.zeros_like(x) if residual is None else residual

@@ -1053,3 +1053,37 @@ def test_grouped_weight_gradient_in_the_weights_type(sizes, n, k):
     assert w.grad.dtype == torch.bfloat16
     assert torch.equal(w.grad, grouped_wgrad(dy, x, offsets).bfloat16())
     check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("buffers", [(), (0,), (1, 2)])
+def test_block_trains_every_weight(buffers):
+    """A weight without a main gradient gets its own, the same fp32 sum rounded once; one with a
+    main gradient does not."""
+    x, wr, wgu, wd = _block(12)
+    weights = (wr, wgu, wd)
+    dout = torch.randn(300, 128, device="cuda").bfloat16()
+    acc = _grads(*weights)
+    fn.moe_swiglu(x.clone().requires_grad_(), *weights, 2, grads=acc).backward(dout)
+    leaves = [w.clone().requires_grad_() for w in weights]
+    into = _grads(*weights)
+    grads = tuple(into[i] if i in buffers else None for i in range(3)) if buffers else None
+    fn.moe_swiglu(x, *leaves, 2, grads=grads).backward(dout)
+    for i, leaf in enumerate(leaves):
+        if i in buffers:
+            assert leaf.grad is None and torch.equal(into[i], acc[i]), i
+        else:
+            assert leaf.grad.dtype == torch.bfloat16 and torch.equal(leaf.grad, acc[i].bfloat16()), i
+            assert not into[i].any()
+    check_device_errors()
+
+
+@gpu
+def test_linear_weight_gets_a_gradient_without_an_accumulator():
+    x = torch.randn(70, 64, device="cuda").bfloat16()
+    w = torch.randn(40, 64, device="cuda").bfloat16().requires_grad_()
+    dy = torch.randn(70, 40, device="cuda").bfloat16()
+    fn.linear(x, w).backward(dy)
+    want, size = dy.double().t() @ x.double(), dy.double().abs().t() @ x.double().abs()
+    assert w.grad.dtype == torch.bfloat16
+    near(w.grad, want, BF * want.abs() + 1.01 * 2 * 70 * F32 * size)
