@@ -56,6 +56,16 @@ int64_t read_and_clear_error(int64_t device_index) {
   return value;
 }
 
+// A message with numbers in it. TORCH_CHECK would format them through a stream, which ends the
+// process here instead of raising (the interpreter and libtorch bring C++ libraries whose stream
+// locales do not fit); std::to_string is safe.
+template <class... Parts>
+static std::string message(const Parts&... parts) {
+  std::string text;
+  detail::append(text, parts...);
+  return text;
+}
+
 static cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream(); }
 
 static void check_cuda_bf16(const torch::Tensor& t, const char* name) {
@@ -76,9 +86,9 @@ void gemm(torch::Tensor a, bool a_mn, torch::Tensor b, bool b_mn, torch::Tensor 
   const int64_t k = a_mn ? a.size(0) : a.size(1);
   const int64_t n = b_mn ? b.size(1) : b.size(0);
   const int64_t kb = b_mn ? b.size(0) : b.size(1);
-  TORCH_CHECK(k == kb, "GEMM reduction sizes differ: ", k, " vs ", kb);
+  TORCH_CHECK(k == kb, message("GEMM reduction sizes differ: ", k, " vs ", kb));
   TORCH_CHECK(c.size(0) == m && c.size(1) == n, "GEMM output shape mismatch");
-  TORCH_CHECK(epi >= 0 && epi <= 4, "unknown GEMM epilogue ", epi);
+  TORCH_CHECK(epi >= 0 && epi <= 4, message("unknown GEMM epilogue ", epi));
   const bool want_f32 = epi == 1 || epi == 2 || epi == 4;
   TORCH_CHECK(c.scalar_type() == (want_f32 ? at::kFloat : at::kBFloat16), "GEMM output dtype does not match epilogue");
   const void* r = nullptr;
@@ -109,7 +119,8 @@ static int sms(const torch::Tensor& t) {
 
 static void check_rows(const torch::Tensor& t, int64_t cols, const char* name) {
   check_cuda_bf16(t, name);
-  TORCH_CHECK(t.dim() == 2 && t.size(1) == cols && t.is_contiguous(), name, " must be contiguous [rows, ", cols, "]");
+  TORCH_CHECK(t.dim() == 2 && t.size(1) == cols && t.is_contiguous(),
+              message(name, " must be contiguous [rows, ", cols, "]"));
 }
 
 // ---- RMSNorm --------------------------------------------------------------------------
@@ -327,7 +338,7 @@ static void check_int32(const torch::Tensor& t, const torch::Tensor& like, const
 }
 
 static void check_rows_count(int64_t rows, int64_t k) {
-  TORCH_CHECK(rows <= kMoeMaxPairs / std::max<int64_t>(k, 1), "tokens * k passes ", kMoeMaxPairs);
+  TORCH_CHECK(rows <= kMoeMaxPairs / std::max<int64_t>(k, 1), message("tokens * k passes ", kMoeMaxPairs));
 }
 
 std::vector<torch::Tensor> moe_route_t(torch::Tensor logits, int64_t k, bool normalize) {

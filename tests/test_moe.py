@@ -1087,3 +1087,39 @@ def test_linear_weight_gets_a_gradient_without_an_accumulator():
     want, size = dy.double().t() @ x.double(), dy.double().abs().t() @ x.double().abs()
     assert w.grad.dtype == torch.bfloat16
     near(w.grad, want, BF * want.abs() + 1.01 * 2 * 70 * F32 * size)
+
+
+_MISFITS = r"""
+import torch
+from resihp.ops import _ext
+from resihp.ops import functional as fn
+
+def bf(*shape):
+    return torch.zeros(*shape, device="cuda", dtype=torch.bfloat16)
+
+ids = torch.zeros(1, 2, dtype=torch.int32, device="cuda").expand(2**30, 2)
+out, k = bf(4, 8), _ext.require()
+calls = (lambda: k.moe_route(torch.zeros(1, 2, device="cuda").expand(2**30, 2), 2, True),
+         lambda: k.moe_scatter(bf(4, 8), ids[0], ids[:4, ::2]),
+         lambda: k.gemm(bf(4, 16), False, bf(8, 24), False, out, 0),
+         lambda: k.gemm(bf(4, 16), False, bf(8, 16), False, out, 9),
+         lambda: k.swiglu_bwd(bf(4, 16), bf(4, 16)))
+for call in calls:
+    try:
+        call()
+    except RuntimeError as error:
+        print("raised", error)
+torch.cuda.synchronize()
+"""
+
+
+@gpu
+def test_refusals_of_the_extension_raise():
+    """A refusal whose message holds numbers is an exception, not the end of the process."""
+    import os
+    import subprocess
+    import sys
+
+    done = subprocess.run([sys.executable, "-c", _MISFITS], capture_output=True, text=True, timeout=600,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0 and done.stdout.count("raised") == 5, (done.stdout, done.stderr[-2000:])
