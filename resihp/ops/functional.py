@@ -240,8 +240,6 @@ def moe_swiglu(x, w_router, w_gate_up, w_down, k, *, normalize=True, residual=No
     autograd. On the kernels the router takes a multiple of 8 experts (its logits are a GEMM's
     output). The steps are :mod:`resihp.ops.moe`'s.
     """
-    if not x.shape[0]:
-        return torch.zeros_like(x) if residual is None else residual
     g_router, g_gate_up, g_down = grads if grads is not None else (None, None, None)
     weights, _, plan = moe_route(linear(x, w_router, g_router), k, normalize)
     gu = grouped_linear(moe_dispatch(x, plan), w_gate_up, plan.offsets, g_gate_up)

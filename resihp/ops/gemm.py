@@ -42,7 +42,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = Non
     lead = x.shape[:-1]
     x2 = x.reshape(-1, x.shape[-1])
     out = torch.empty((x2.shape[0], w.shape[0]), dtype=torch.bfloat16, device=x.device)
-    if residual is None:
+    if not out.shape[0]:  # no rows: nothing to launch
+        pass
+    elif residual is None:
         _ext.require().gemm(x2, False, w, False, out, EPI_BF16)
     else:
         r2 = residual.reshape(-1, w.shape[0])
@@ -57,7 +59,8 @@ def linear_dgrad(dy: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     lead = dy.shape[:-1]
     d2 = dy.reshape(-1, dy.shape[-1])
     out = torch.empty((d2.shape[0], w.shape[1]), dtype=torch.bfloat16, device=dy.device)
-    _ext.require().gemm(d2, False, w, True, out, EPI_BF16)
+    if out.shape[0]:
+        _ext.require().gemm(d2, False, w, True, out, EPI_BF16)
     return out.view(*lead, w.shape[1])
 
 
@@ -82,6 +85,8 @@ def linear_wgrad(dy: torch.Tensor, x: torch.Tensor, out: torch.Tensor | None = N
     if out is None:
         out = torch.empty((d2.shape[1], x2.shape[1]), dtype=torch.float32, device=dy.device)
         accumulate = False
+    if not d2.shape[0]:  # no rows: a sum of nothing
+        return out if accumulate else out.zero_()
     _ext.require().gemm(d2, True, x2, True, out, ((EPI_RED_F32 if WGRAD_RED else EPI_ACC_F32) if accumulate
                                                  else EPI_F32))
     return out

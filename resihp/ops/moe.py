@@ -162,8 +162,7 @@ def moe_combine(y, weights, plan: MoePlan, residual=None):
         return _ext.require().moe_combine_ad(y, weights, offsets, slots, residual)
     at = slots.long()
     kept = ((at >= 0) & (at < offsets[-1].clamp_max(at.numel())))[..., None]
-    rows = y[torch.where(kept[..., 0], at, torch.zeros_like(at)).reshape(-1)].view(*at.shape, -1) if at.numel() else \
-        y.new_zeros(*at.shape, y.shape[1])
+    rows = y[torch.where(kept[..., 0], at, torch.zeros_like(at)).reshape(-1)].view(*at.shape, y.shape[1])
     out = (torch.where(kept, rows, torch.zeros((), dtype=y.dtype, device=y.device)) * weights[..., None]).sum(1)
     return (out if residual is None else residual + out).to(y.dtype)
 

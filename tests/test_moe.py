@@ -1123,3 +1123,28 @@ def test_refusals_of_the_extension_raise():
     done = subprocess.run([sys.executable, "-c", _MISFITS], capture_output=True, text=True, timeout=600,
                           cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert done.returncode == 0 and done.stdout.count("raised") == 5, (done.stdout, done.stderr[-2000:])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_block_without_tokens_stays_in_the_graph(device, with_residual):
+    """A rank that got no tokens: the output is a new tensor, and every leaf gets zeros."""
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    leaves = [torch.randn(s, device=device).to(dtype).requires_grad_() for s in ((0, 16), (8, 16), (8, 48, 16), (8, 16, 24))]
+    residual = torch.zeros(0, 16, device=device, dtype=dtype).requires_grad_() if with_residual else None
+    out = fn.moe_swiglu(*leaves, 2, residual=residual)
+    assert out.shape == (0, 16) and out is not residual and not out.is_leaf
+    out.sum().backward()
+    for leaf in leaves + ([residual] if with_residual else []):
+        assert leaf.grad.shape == leaf.shape and not leaf.grad.any()
+
+
+@gpu
+def test_linear_products_without_rows():
+    x, w = torch.empty(0, 16, device="cuda").bfloat16(), torch.randn(24, 16, device="cuda").bfloat16()
+    dy = torch.empty(0, 24, device="cuda").bfloat16()
+    assert fn.linear(x, w).shape == fn.linear(x, w, residual=dy).shape == (0, 24)
+    assert fn.linear_dgrad(dy, w).shape == (0, 16)
+    assert torch.equal(fn.linear_wgrad(dy, x), torch.zeros(24, 16, device="cuda"))
+    kept = torch.ones(24, 16, device="cuda")
+    assert fn.linear_wgrad(dy, x, out=kept, accumulate=True).all() and not fn.linear_wgrad(dy, x, out=kept).any()
