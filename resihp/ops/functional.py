@@ -28,7 +28,7 @@ from . import _ext
 from .gemm import linear as _gemm_linear
 from .gemm import grouped_dgrad, grouped_wgrad, linear_dgrad, linear_wgrad  # noqa: F401
 from .dropout import dropout  # noqa: F401
-from .moe import MoePlan, grouped_linear, moe_combine, moe_dispatch, moe_plan, moe_route  # noqa: F401
+from .moe import MoePlan, check_block, grouped_linear, moe_combine, moe_dispatch, moe_plan, moe_route  # noqa: F401
 
 
 def _k():
@@ -240,6 +240,7 @@ def moe_swiglu(x, w_router, w_gate_up, w_down, k, *, normalize=True, residual=No
     autograd. On the kernels the router takes a multiple of 8 experts (its logits are a GEMM's
     output). The steps are :mod:`resihp.ops.moe`'s.
     """
+    check_block(x, w_router, w_gate_up, w_down, k, residual, grads)
     g_router, g_gate_up, g_down = grads if grads is not None else (None, None, None)
     weights, _, plan = moe_route(linear(x, w_router, g_router), k, normalize)
     gu = grouped_linear(moe_dispatch(x, plan), w_gate_up, plan.offsets, g_gate_up)

@@ -75,6 +75,12 @@ def _route_torch(logits, k: int, normalize: bool):
     return weights, torch.where(allowed, ids, torch.full_like(ids, -1)).to(torch.int32)
 
 
+def _check_choices(experts: int, k: int) -> None:
+    if not 1 <= experts <= MAX_GROUPS or not 1 <= k <= min(experts, MAX_CHOICES):
+        raise ValueError(f"{k} choices of {experts} experts: 1 to {MAX_CHOICES} choices, no more than experts, "
+                         f"of 1 to {MAX_GROUPS} experts")
+
+
 def moe_route(logits, k: int, normalize: bool = True):
     """The ``k`` experts of every token: ``(weights, ids, plan)`` from router logits ``[T, E]``.
 
@@ -89,9 +95,7 @@ def moe_route(logits, k: int, normalize: bool = True):
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"router logits must be bf16 or fp32 [T, E], got {logits.dtype} {list(logits.shape)}")
     experts = logits.shape[1]
-    if not 1 <= experts <= MAX_GROUPS or not 1 <= k <= min(experts, MAX_CHOICES):
-        raise ValueError(f"{k} choices of {experts} experts: 1 to {MAX_CHOICES} choices, no more than experts, "
-                         f"of 1 to {MAX_GROUPS} experts")
+    _check_choices(experts, k)
     if logits.is_cuda:
         weights, ids, offsets, slots = _ext.require().moe_route_ad(logits, k, normalize)
         return weights, ids, MoePlan(offsets, slots)
@@ -187,3 +191,35 @@ def grouped_linear(x, w, offsets, main_grad=None):
     if not _cuda(x):
         return _grouped_linear(x, w, offsets)
     return _ext.require().grouped_linear_ad(x, w, offsets.contiguous(), main_grad)
+
+
+def check_block(x, w_router, w_gate_up, w_down, k: int, residual, grads) -> None:
+    """Refuse operands of a sparse block before its first step is launched."""
+    if x.dim() != 2 or w_router.dim() != 2 or w_gate_up.dim() != 3 or w_down.dim() != 3:
+        raise ValueError("a sparse block takes x [T, d], w_router [E, d], w_gate_up [E, 2F, d] and w_down [E, d, F]")
+    (experts, d), f = w_router.shape, w_down.shape[2]
+    if x.shape[1] != d or w_gate_up.shape != (experts, 2 * f, d) or w_down.shape != (experts, d, f) or d < 1 or f < 1:
+        raise ValueError(f"x {list(x.shape)}, w_router {list(w_router.shape)}, w_gate_up {list(w_gate_up.shape)} and "
+                         f"w_down {list(w_down.shape)} are not [T, d], [E, d], [E, 2F, d] and [E, d, F]")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"a sparse block runs in bf16 or fp32, not {x.dtype}")
+    weights = (w_router, w_gate_up, w_down)
+    if any(w.dtype != x.dtype or w.device != x.device for w in weights):
+        raise ValueError(f"the weights must match x ({x.dtype}, {x.device})")
+    _check_choices(experts, k)
+    if _cuda(x) and (experts % 8 or d % 8 or f % 8):
+        raise ValueError(f"the bf16 kernels need experts and widths that are multiples of 8, got {experts} experts, "
+                         f"{d} and {f}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("the residual must match x in shape, dtype and device")
+    if grads is None:
+        return
+    if len(grads) != 3:
+        raise ValueError("grads are the main gradients of the router's, gate / up's and down's weights")
+    for w, g in zip(weights, grads):
+        if g is not None and (g.shape != w.shape or g.dtype != torch.float32 or g.device != w.device):
+            raise ValueError(f"main gradients must be fp32 {list(w.shape)} beside their weights")
+        if g is not None and _cuda(w) and (g.stride(-1) != 1 or g.data_ptr() % 16 or g.stride(0) % 8):
+            raise ValueError("main gradients must be 16-byte aligned rows")
+        if g is not None and w.dim() == 3 and not g.is_contiguous():
+            raise ValueError("the experts' main gradients must be contiguous")

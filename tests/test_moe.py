@@ -1148,3 +1148,76 @@ def test_linear_products_without_rows():
     assert torch.equal(fn.linear_wgrad(dy, x), torch.zeros(24, 16, device="cuda"))
     kept = torch.ones(24, 16, device="cuda")
     assert fn.linear_wgrad(dy, x, out=kept, accumulate=True).all() and not fn.linear_wgrad(dy, x, out=kept).any()
+
+
+def _fp32_block(d, x=(4, 16), router=(8, 16), gate_up=(8, 48, 16), down=(8, 16, 24), dtype=torch.float32):
+    return [torch.zeros(s, device=d, dtype=dtype) for s in (x, router, gate_up, down)]
+
+
+BLOCK_REFUSALS = {
+    "flat rows": lambda d: fn.moe_swiglu(*_fp32_block(d, x=(16,)), 2),
+    "rows of a batch": lambda d: fn.moe_swiglu(*_fp32_block(d, x=(2, 4, 16)), 2),
+    "rows of another width": lambda d: fn.moe_swiglu(*_fp32_block(d, x=(4, 24)), 2),
+    "a router of another width": lambda d: fn.moe_swiglu(*_fp32_block(d, router=(8, 24)), 2),
+    "gate and up of another count": lambda d: fn.moe_swiglu(*_fp32_block(d, gate_up=(7, 48, 16)), 2),
+    "gate and up of an odd height": lambda d: fn.moe_swiglu(*_fp32_block(d, gate_up=(8, 49, 16)), 2),
+    "down of another width": lambda d: fn.moe_swiglu(*_fp32_block(d, down=(8, 16, 16)), 2),
+    "down of another height": lambda d: fn.moe_swiglu(*_fp32_block(d, down=(8, 24, 24)), 2),
+    "two-dimensional weights": lambda d: fn.moe_swiglu(*_fp32_block(d, down=(16, 24)), 2),
+    "half precision": lambda d: fn.moe_swiglu(*_fp32_block(d, dtype=torch.float16), 2),
+    "types that differ": lambda d: fn.moe_swiglu(torch.zeros(4, 16, device=d).bfloat16(), *_fp32_block(d)[1:], 2),
+    "more choices than experts": lambda d: fn.moe_swiglu(*_fp32_block(d), 9),
+    "no choice": lambda d: fn.moe_swiglu(*_fp32_block(d), 0),
+    "a residual of another shape": lambda d: fn.moe_swiglu(*_fp32_block(d), 2, residual=torch.zeros(1, 16, device=d)),
+    "a residual of another type": lambda d: fn.moe_swiglu(*_fp32_block(d), 2, residual=torch.zeros(4, 16, device=d).bfloat16()),
+    "two accumulators": lambda d: fn.moe_swiglu(*_fp32_block(d), 2, grads=_fp32_block(d)[1:3]),
+    "a router's accumulator of another shape": lambda d: fn.moe_swiglu(
+        *_fp32_block(d), 2, grads=(torch.zeros(16, 8, device=d), None, None)),
+    "an accumulator of another type": lambda d: fn.moe_swiglu(
+        *_fp32_block(d), 2, grads=(None, None, torch.zeros(8, 16, 24, device=d).bfloat16())),
+    "an accumulator with gaps": lambda d: fn.moe_swiglu(
+        *_fp32_block(d), 2, grads=(None, torch.zeros(8, 48, 32, device=d)[..., :16], None)),
+}
+KERNEL_BLOCK_REFUSALS = {
+    "12 experts": dict(router=(12, 16), gate_up=(12, 48, 16), down=(12, 16, 24)),
+    "rows of width 20": dict(x=(4, 20), router=(8, 20), gate_up=(8, 48, 20), down=(8, 20, 24)),
+    "an inner width of 20": dict(gate_up=(8, 40, 16), down=(8, 16, 20)),
+}
+
+
+@pytest.mark.parametrize("what", sorted(BLOCK_REFUSALS))
+def test_block_refusals(what):
+    with pytest.raises(ValueError):
+        BLOCK_REFUSALS[what]("cpu")
+
+
+@gpu
+@pytest.mark.parametrize("what", sorted(BLOCK_REFUSALS))
+def test_block_refusals_on_the_gpu(what):
+    with pytest.raises(ValueError):
+        BLOCK_REFUSALS[what]("cuda")
+
+
+@gpu
+@pytest.mark.parametrize("what", sorted(KERNEL_BLOCK_REFUSALS))
+def test_block_refusals_of_the_kernels(what):
+    """Before anything is launched; fp32 takes the same sizes."""
+    from resihp.ops import _ext
+
+    counter = _ext.launch_counter()
+    before, (counter.launches, counter.enabled) = (counter.launches, counter.enabled), (0, True)
+    try:
+        with pytest.raises(ValueError, match="multiples of 8"):
+            fn.moe_swiglu(*_fp32_block("cuda", dtype=torch.bfloat16, **KERNEL_BLOCK_REFUSALS[what]), 2)
+        assert counter.launches == 0
+    finally:
+        counter.launches, counter.enabled = before
+    assert fn.moe_swiglu(*_fp32_block("cuda", **KERNEL_BLOCK_REFUSALS[what]), 2).shape[0] == 4
+
+
+@gpu
+def test_block_refuses_a_router_accumulator_off_16_bytes():
+    x, wr, wgu, wd = _block(13)
+    odd = torch.zeros(8 * 128 + 1, device="cuda")[1:].view(8, 128)
+    with pytest.raises(ValueError, match="aligned"):
+        fn.moe_swiglu(x, wr, wgu, wd, 2, grads=(odd, None, None))
