@@ -26,7 +26,7 @@ from torch.nn import functional as F
 
 from . import _ext
 from .gemm import linear as _gemm_linear
-from .gemm import grouped_dgrad, grouped_wgrad, linear_dgrad, linear_wgrad  # noqa: F401
+from .gemm import _tiles, grouped_dgrad, grouped_wgrad, linear_dgrad, linear_wgrad  # noqa: F401
 from .dropout import dropout  # noqa: F401
 from .moe import MoePlan, check_block, grouped_linear, moe_combine, moe_dispatch, moe_plan, moe_route  # noqa: F401
 
@@ -242,7 +242,11 @@ def moe_swiglu(x, w_router, w_gate_up, w_down, k, *, normalize=True, residual=No
     """
     check_block(x, w_router, w_gate_up, w_down, k, residual, grads)
     g_router, g_gate_up, g_down = grads if grads is not None else (None, None, None)
-    weights, _, plan = moe_route(linear(x, w_router, g_router), k, normalize)
+    if on_kernels(x):  # any view: the router's product reads its operands through TMA, as the experts' do
+        logits = linear(_tiles(x), _tiles(w_router), g_router)
+    else:
+        logits = linear(x, w_router)
+    weights, _, plan = moe_route(logits, k, normalize)
     gu = grouped_linear(moe_dispatch(x, plan), w_gate_up, plan.offsets, g_gate_up)
     y = grouped_linear(swiglu(gu), w_down, plan.offsets, g_down)
     return moe_combine(y, weights, plan, residual)

@@ -1221,3 +1221,23 @@ def test_block_refuses_a_router_accumulator_off_16_bytes():
     odd = torch.zeros(8 * 128 + 1, device="cuda")[1:].view(8, 128)
     with pytest.raises(ValueError, match="aligned"):
         fn.moe_swiglu(x, wr, wgu, wd, 2, grads=(odd, None, None))
+
+
+@gpu
+def test_block_takes_views():
+    """Rows and router weights at odd addresses, strided and transposed, as the other steps take them."""
+    x, wr, wgu, wd = _block(14)
+    want = fn.moe_swiglu(x, wr, wgu, wd, 2)
+    odd = torch.empty(x.numel() + 3, device="cuda", dtype=torch.bfloat16)[3:].view(300, 128).copy_(x)
+    wide = torch.zeros(300, 133, device="cuda", dtype=torch.bfloat16)
+    wide[:, 5:] = x
+    views = (odd, wide[:, 5:], x.t().contiguous().t())
+    router = wr.t().contiguous().t()
+    for view in views:
+        assert torch.equal(fn.moe_swiglu(view, router, wgu, wd, 2), want)
+    leaf, wleaf = x.t().contiguous().requires_grad_(), wr.t().contiguous().requires_grad_()
+    fn.moe_swiglu(leaf.t(), wleaf.t(), wgu, wd, 2).backward(want)
+    xr, wrr = x.clone().requires_grad_(), wr.clone().requires_grad_()
+    fn.moe_swiglu(xr, wrr, wgu, wd, 2).backward(want)
+    assert torch.equal(leaf.grad.t(), xr.grad) and torch.equal(wleaf.grad.t(), wrr.grad)
+    check_device_errors()
