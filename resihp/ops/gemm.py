@@ -125,6 +125,12 @@ def _check_widths(x: torch.Tensor, n: int, k: int) -> None:
         raise ValueError(f"grouped products run in bf16 or fp32, not {x.dtype}")
 
 
+def check_aligned(rows: torch.Tensor, out: torch.Tensor) -> None:
+    """The kernels write a weight gradient in 16-byte units."""
+    if _cuda(rows) and out.data_ptr() % 16:
+        raise ValueError("the bf16 kernels need a weight gradient at a 16-byte aligned address")
+
+
 def _tiles(t: torch.Tensor) -> torch.Tensor:
     """``t`` as TMA reads it: unit inner stride, 16-byte aligned base and outer strides (which
     no two rows may share); anything else is copied."""
@@ -180,6 +186,8 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out:
         out, accumulate = torch.empty(shape, dtype=torch.float32, device=dy.device), False
     elif out.shape != shape or out.dtype != torch.float32 or out.device != dy.device or not out.is_contiguous():
         raise ValueError(f"the weight gradient goes into a contiguous fp32 {list(shape)} on the rows' device")
+    else:
+        check_aligned(dy, out)
     if _cuda(dy):
         _ext.require().grouped_wgrad(_tiles(dy), _tiles(x), offsets.contiguous(), out, accumulate)
         return out

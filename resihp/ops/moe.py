@@ -26,7 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _ext
-from .gemm import MAX_GROUPS, _cuda, check_groups
+from .gemm import MAX_GROUPS, _cuda, check_aligned, check_groups
 from .gemm import grouped_linear as _grouped_linear
 
 MAX_CHOICES = 16
@@ -188,6 +188,8 @@ def grouped_linear(x, w, offsets, main_grad=None):
     if main_grad is not None and (main_grad.shape != w.shape or main_grad.dtype != torch.float32
                                   or main_grad.device != w.device or not main_grad.is_contiguous()):
         raise ValueError(f"main_grad must be a contiguous fp32 {list(w.shape)} beside the weights")
+    if main_grad is not None:
+        check_aligned(x, main_grad)
     if not _cuda(x):
         return _grouped_linear(x, w, offsets)
     return _ext.require().grouped_linear_ad(x, w, offsets.contiguous(), main_grad)

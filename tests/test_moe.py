@@ -1241,3 +1241,18 @@ def test_block_takes_views():
     fn.moe_swiglu(xr, wrr, wgu, wd, 2).backward(want)
     assert torch.equal(leaf.grad.t(), xr.grad) and torch.equal(wleaf.grad.t(), wrr.grad)
     check_device_errors()
+
+
+@gpu
+def test_weight_gradients_off_16_bytes_are_refused():
+    """Before the forward pass, not in the backward pass; fp32 rows take such an accumulator."""
+    x, w, dy, offsets = _grouped_case([3, 6], 0, 16, 24)
+    odd = torch.zeros(w.numel() + 1, device="cuda")[1:].view(w.shape)
+    with pytest.raises(ValueError, match="aligned"):
+        fn.grouped_linear(x.requires_grad_(), w, offsets, main_grad=odd)
+    with pytest.raises(ValueError, match="aligned"):
+        grouped_wgrad(dy, x.detach(), offsets, out=odd, accumulate=True)
+    assert not odd.any()
+    grouped_wgrad(dy.float(), x.detach().float(), offsets, out=odd)
+    near(odd, grouped_wgrad(dy, x.detach(), offsets), 1e-4)
+    check_device_errors()
