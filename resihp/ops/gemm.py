@@ -97,6 +97,7 @@ def linear_wgrad(dy: torch.Tensor, x: torch.Tensor, out: torch.Tensor | None = N
 # ---------------------------------------------------------------------------------------
 
 MAX_GROUPS = 1024
+MAX_SIZE = 2**31 - 1 - 512  # rows and widths: leaves room for a tile in 31 bits
 
 
 def check_groups(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> None:
@@ -121,6 +122,8 @@ def _check_widths(x: torch.Tensor, n: int, k: int) -> None:
         raise ValueError("a grouped product needs widths of at least 1")
     if _cuda(x) and (n % 8 or k % 8):
         raise ValueError(f"the bf16 kernels need widths that are multiples of 8, got {n} and {k}")
+    if _cuda(x) and max(x.shape[0], n, k) > MAX_SIZE:
+        raise ValueError(f"the bf16 kernels take up to {MAX_SIZE} rows and columns, got {x.shape[0]}, {n} and {k}")
     if x.is_cuda and x.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"grouped products run in bf16 or fp32, not {x.dtype}")
 

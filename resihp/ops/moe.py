@@ -30,6 +30,7 @@ from .gemm import MAX_GROUPS, _cuda, check_aligned, check_groups
 from .gemm import grouped_linear as _grouped_linear
 
 MAX_CHOICES = 16
+MAX_PAIRS = 0x7FFF0000  # tokens * k: places are int32, with room for a block's rows
 
 
 class MoePlan(NamedTuple):
@@ -75,6 +76,11 @@ def _route_torch(logits, k: int, normalize: bool):
     return weights, torch.where(allowed, ids, torch.full_like(ids, -1)).to(torch.int32)
 
 
+def _check_pairs(tokens: int, k: int) -> None:
+    if tokens * k > MAX_PAIRS:
+        raise ValueError(f"a plan takes up to {MAX_PAIRS} (token, choice) pairs, got {tokens} x {k}")
+
+
 def _check_choices(experts: int, k: int) -> None:
     if not 1 <= experts <= MAX_GROUPS or not 1 <= k <= min(experts, MAX_CHOICES):
         raise ValueError(f"{k} choices of {experts} experts: 1 to {MAX_CHOICES} choices, no more than experts, "
@@ -96,6 +102,7 @@ def moe_route(logits, k: int, normalize: bool = True):
         raise ValueError(f"router logits must be bf16 or fp32 [T, E], got {logits.dtype} {list(logits.shape)}")
     experts = logits.shape[1]
     _check_choices(experts, k)
+    _check_pairs(logits.shape[0], k)
     if logits.is_cuda:
         weights, ids, offsets, slots = _ext.require().moe_route_ad(logits, k, normalize)
         return weights, ids, MoePlan(offsets, slots)
@@ -110,6 +117,7 @@ def moe_plan(ids, experts: int, start: int = 0) -> MoePlan:
         raise ValueError(f"expert ids must be int32 [T, k], got {ids.dtype} {list(ids.shape)}")
     if not 1 <= experts <= MAX_GROUPS or not -(2**31) <= start < 2**31:
         raise ValueError(f"a plan takes 1 to {MAX_GROUPS} experts from a 32-bit start, got {experts} from {start}")
+    _check_pairs(*ids.shape)
     if ids.is_cuda:
         return MoePlan(*_ext.require().moe_plan(ids.contiguous(), int(experts), int(start)))
     return _plan_torch(ids, experts, start)
@@ -124,6 +132,7 @@ def _check_plan(rows, plan: MoePlan) -> tuple[torch.Tensor, torch.Tensor]:
     offsets, slots = plan
     if slots.dim() != 2 or slots.shape[1] < 1 or offsets.dim() != 1 or offsets.numel() < 2:
         raise ValueError("a plan is offsets [E + 1] and slots [T, k]")
+    _check_pairs(*slots.shape)
     if slots.dtype != torch.int32 or offsets.dtype != torch.int32:
         raise ValueError("a plan's offsets and slots must be int32")
     if slots.device != rows.device or offsets.device != rows.device:
@@ -209,6 +218,7 @@ def check_block(x, w_router, w_gate_up, w_down, k: int, residual, grads) -> None
     if any(w.dtype != x.dtype or w.device != x.device for w in weights):
         raise ValueError(f"the weights must match x ({x.dtype}, {x.device})")
     _check_choices(experts, k)
+    _check_pairs(x.shape[0], k)
     if _cuda(x) and (experts % 8 or d % 8 or f % 8):
         raise ValueError(f"the bf16 kernels need experts and widths that are multiples of 8, got {experts} experts, "
                          f"{d} and {f}")

@@ -1256,3 +1256,40 @@ def test_weight_gradients_off_16_bytes_are_refused():
     grouped_wgrad(dy.float(), x.detach().float(), offsets, out=odd)
     near(odd, grouped_wgrad(dy, x.detach(), offsets), 1e-4)
     check_device_errors()
+
+
+def _many(d, *shape, dtype=torch.float32):
+    """2^30 rows or more that are one row."""
+    return torch.zeros(1, *shape[1:], device=d, dtype=dtype).expand(*shape)
+
+
+SIZE_REFUSALS = {
+    "logits": lambda d: fn.moe_route(_many(d, 2**30, 2), 2),
+    "ids": lambda d: fn.moe_plan(_many(d, 2**30, 2, dtype=torch.int32), 4),
+    "a plan of rows": lambda d: fn.moe_dispatch(_many(d, 2**30, 8), fn.MoePlan(ragged([4], d), _many(d, 2**30, 2, dtype=torch.int32))),
+    "a plan of expert rows": lambda d: fn.moe_combine(
+        _many(d, 2**31, 8), _many(d, 2**30, 2), fn.MoePlan(ragged([4], d), _many(d, 2**30, 2, dtype=torch.int32))),
+    "a block": lambda d: fn.moe_swiglu(_many(d, 2**30, 16), *_fp32_block(d)[1:], 2),
+}
+
+
+@pytest.mark.parametrize("what", sorted(SIZE_REFUSALS))
+def test_refusals_of_more_pairs_than_31_bits_count(what):
+    with pytest.raises(ValueError, match="pairs"):
+        SIZE_REFUSALS[what]("cpu")
+
+
+@gpu
+@pytest.mark.parametrize("what", sorted(SIZE_REFUSALS))
+def test_refusals_of_more_pairs_than_31_bits_count_on_the_gpu(what):
+    with pytest.raises(ValueError, match="pairs"):
+        SIZE_REFUSALS[what]("cuda")
+
+
+@gpu
+def test_refusals_of_more_rows_than_31_bits_count():
+    x, w = _many("cuda", 2**31, 8, dtype=torch.bfloat16), torch.zeros(1, 8, 8, device="cuda").bfloat16()
+    for call in (lambda: fn.grouped_linear(x, w, ragged([4], "cuda")), lambda: grouped_dgrad(x, w, ragged([4], "cuda")),
+                 lambda: grouped_wgrad(x, x, ragged([4], "cuda"))):
+        with pytest.raises(ValueError, match="rows and columns"):
+            call()
