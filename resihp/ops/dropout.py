@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext
+from .gemm import whole
 
 _M32 = 0xFFFFFFFF
 
@@ -68,19 +69,25 @@ def dropout(x, p: float, seed, offset: int = 0, residual=None, first_row: int = 
     whole tensor (a token shard draws its part of that tensor's mask); rows are the last
     dimension of ``x``. A dropped infinity or NaN gives 0.
     """
+    try:
+        p = float(p * 1.0)  # (a number's product; a text has none)
+    except (TypeError, OverflowError):
+        raise ValueError(f"dropout probability must be a number, got {p!r}") from None
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability must lie in [0, 1], got {p}")
     if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() < 1:
         raise ValueError(f"dropout takes bf16 or fp32 rows, got {x.dtype} {list(x.shape)}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("the residual must match x in shape, dtype and device")
-    state = None
+    offset, first_row, state = whole(offset, "the offset"), whole(first_row, "first_row"), None
     if torch.is_tensor(seed):
         if seed.dtype != torch.int64 or seed.shape != (2,) or seed.device != x.device or offset:
             raise ValueError("a seed tensor is int64 [seed, offset] beside x, with no other offset")
         state, seed = seed.contiguous(), 0
-    elif not 0 <= seed < 1 << 64:
-        raise ValueError("the seed must be an unsigned 64-bit number")
+    else:
+        seed = whole(seed, "the seed")
+        if not 0 <= seed < 1 << 64:
+            raise ValueError("the seed must be an unsigned 64-bit number")
     if not 0 <= offset < 1 << 64:
         raise ValueError("the offset must be an unsigned 64-bit number")
     first = first_row * x.shape[-1]

@@ -26,7 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _ext
-from .gemm import MAX_GROUPS, _cuda, check_aligned, check_groups
+from .gemm import MAX_GROUPS, _cuda, check_aligned, check_groups, whole
 from .gemm import grouped_linear as _grouped_linear
 
 MAX_CHOICES = 16
@@ -81,10 +81,12 @@ def _check_pairs(tokens: int, k: int) -> None:
         raise ValueError(f"a plan takes up to {MAX_PAIRS} (token, choice) pairs, got {tokens} x {k}")
 
 
-def _check_choices(experts: int, k: int) -> None:
+def _check_choices(experts: int, k) -> int:
+    k = whole(k, "the number of choices")
     if not 1 <= experts <= MAX_GROUPS or not 1 <= k <= min(experts, MAX_CHOICES):
         raise ValueError(f"{k} choices of {experts} experts: 1 to {MAX_CHOICES} choices, no more than experts, "
                          f"of 1 to {MAX_GROUPS} experts")
+    return k
 
 
 def moe_route(logits, k: int, normalize: bool = True):
@@ -101,7 +103,7 @@ def moe_route(logits, k: int, normalize: bool = True):
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"router logits must be bf16 or fp32 [T, E], got {logits.dtype} {list(logits.shape)}")
     experts = logits.shape[1]
-    _check_choices(experts, k)
+    k = _check_choices(experts, k)
     _check_pairs(logits.shape[0], k)
     if logits.is_cuda:
         weights, ids, offsets, slots = _ext.require().moe_route_ad(logits, k, normalize)
@@ -115,11 +117,12 @@ def moe_plan(ids, experts: int, start: int = 0) -> MoePlan:
     start + experts`` (this rank's); any other id is a choice that no expert here takes."""
     if ids.dim() != 2 or ids.dtype != torch.int32 or ids.shape[1] < 1:
         raise ValueError(f"expert ids must be int32 [T, k], got {ids.dtype} {list(ids.shape)}")
+    experts, start = whole(experts, "the number of experts"), whole(start, "the first expert")
     if not 1 <= experts <= MAX_GROUPS or not -(2**31) <= start < 2**31:
         raise ValueError(f"a plan takes 1 to {MAX_GROUPS} experts from a 32-bit start, got {experts} from {start}")
     _check_pairs(*ids.shape)
     if ids.is_cuda:
-        return MoePlan(*_ext.require().moe_plan(ids.contiguous(), int(experts), int(start)))
+        return MoePlan(*_ext.require().moe_plan(ids.contiguous(), experts, start))
     return _plan_torch(ids, experts, start)
 
 
@@ -217,8 +220,7 @@ def check_block(x, w_router, w_gate_up, w_down, k: int, residual, grads) -> None
     weights = (w_router, w_gate_up, w_down)
     if any(w.dtype != x.dtype or w.device != x.device for w in weights):
         raise ValueError(f"the weights must match x ({x.dtype}, {x.device})")
-    _check_choices(experts, k)
-    _check_pairs(x.shape[0], k)
+    _check_pairs(x.shape[0], _check_choices(experts, k))
     if _cuda(x) and (experts % 8 or d % 8 or f % 8):
         raise ValueError(f"the bf16 kernels need experts and widths that are multiples of 8, got {experts} experts, "
                          f"{d} and {f}")

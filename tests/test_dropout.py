@@ -257,3 +257,29 @@ def test_gradient_against_differences(dtype):
         size = abs(moved[r, c].item()) + abs(x[r, c].item())
         assert abs(diff - leaf.grad[r, c].item() * step) <= 4 * HALF[dtype] * (size + h) * 65536 / (65536 - 16384)
         assert (leaf.grad[r, c] != 0).item() == keep[r, c].item()
+
+
+NOT_NUMBERS = {
+    "a fractional seed": lambda x: fn.dropout(x, 0.5, 1.5),
+    "a seed of text": lambda x: fn.dropout(x, 0.5, "1"),
+    "a fractional offset": lambda x: fn.dropout(x, 0.5, 1, 2.5),
+    "a fractional row": lambda x: fn.dropout(x, 0.5, 1, first_row=1.0),
+    "p of text": lambda x: fn.dropout(x, "0.5", 1),
+    "no p": lambda x: fn.dropout(x, None, 1),
+}
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("what", sorted(NOT_NUMBERS))
+def test_refusals_of_what_is_no_number(what, device):
+    with pytest.raises(ValueError, match="number"):
+        NOT_NUMBERS[what](torch.zeros(2, 8, device=device))
+
+
+def test_numbers_of_any_type():
+    import numpy as np
+
+    x = torch.ones(4, 9)
+    want = fn.dropout(x, 0.25, 3, 4, first_row=2)
+    assert torch.equal(fn.dropout(x, np.float64(0.25), np.uint64(3), np.int32(4), first_row=np.int64(2)), want)
+    assert torch.equal(fn.dropout(x, np.float32(0.25), True + 2, 4, first_row=2), want)

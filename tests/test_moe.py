@@ -1293,3 +1293,12 @@ def test_refusals_of_more_rows_than_31_bits_count():
                  lambda: grouped_wgrad(x, x, ragged([4], "cuda"))):
         with pytest.raises(ValueError, match="rows and columns"):
             call()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_refusals_of_counts_that_are_not_whole(device):
+    logits, ids = torch.zeros(4, 8, device=device), torch.zeros(4, 2, dtype=torch.int32, device=device)
+    for call in (lambda: fn.moe_route(logits, 2.0), lambda: fn.moe_route(logits, "2"), lambda: fn.moe_plan(ids, 4.0),
+                 lambda: fn.moe_plan(ids, 4, start=0.5), lambda: fn.moe_swiglu(*_fp32_block(device), 2.0)):
+        with pytest.raises(ValueError, match="whole number"):
+            call()
