@@ -566,7 +566,8 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
 
 struct RouteNode : torch::autograd::Function<RouteNode> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, int64_t k, bool normalize) {
-    const auto rows = logits.stride(1) == 1 ? logits : logits.contiguous();
+    // (a copy, not contiguous(): that leaves a single column's stride as it is)
+    const auto rows = logits.stride(1) == 1 ? logits : torch::empty(logits.sizes(), logits.options()).copy_(logits);
     auto out = moe_route_t(rows, k, normalize);
     ctx->mark_non_differentiable({out[1], out[2], out[3]});
     ctx->set_materialize_grads(false);

@@ -1302,3 +1302,17 @@ def test_refusals_of_counts_that_are_not_whole(device):
                  lambda: fn.moe_plan(ids, 4, start=0.5), lambda: fn.moe_swiglu(*_fp32_block(device), 2.0)):
         with pytest.raises(ValueError, match="whole number"):
             call()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_route_takes_one_expert_with_strides(dtype):
+    row = torch.randn(1, 37, device="cuda").to(dtype)
+    row[0, 3] = NINF
+    leaf = row.clone().requires_grad_()
+    weights, ids, plan = fn.moe_route(leaf.t(), 1)
+    want = fn.moe_route(row.t().clone(memory_format=torch.contiguous_format).reshape(-1, 1), 1)
+    assert torch.equal(weights, want[0]) and torch.equal(ids, want[1]) and torch.equal(plan.slots, want[2].slots)
+    assert ids[3] == -1 and weights.sum() == 36 and plan.offsets.tolist() == [0, 36]
+    weights.backward(torch.randn_like(weights))
+    assert not leaf.grad.any()  # the only expert's weight is 1 whatever its logit
