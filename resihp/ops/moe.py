@@ -72,7 +72,8 @@ def _route_torch(logits, k: int, normalize: bool):
     m = among.amax(1, keepdim=True).detach()
     m = torch.where(m == float("-inf"), torch.zeros_like(m), m)
     total = (among - m).exp().sum(1, keepdim=True)
-    weights = torch.where(allowed, (top - m).exp(), torch.zeros_like(top)) / total.masked_fill(total == 0, 1.0)
+    # (chosen after the division: a gradient at a choice that was not made does not reach ``total``)
+    weights = torch.where(allowed, (top - m).exp() / total.masked_fill(total == 0, 1.0), torch.zeros_like(top))
     return weights, torch.where(allowed, ids, torch.full_like(ids, -1)).to(torch.int32)
 
 
@@ -179,7 +180,8 @@ def moe_combine(y, weights, plan: MoePlan, residual=None):
     at = slots.long()
     kept = ((at >= 0) & (at < offsets[-1].clamp_max(at.numel())))[..., None]
     rows = y[torch.where(kept[..., 0], at, torch.zeros_like(at)).reshape(-1)].view(*at.shape, y.shape[1])
-    out = (torch.where(kept, rows, torch.zeros((), dtype=y.dtype, device=y.device)) * weights[..., None]).sum(1)
+    zero = torch.zeros((), device=y.device)  # (in both factors: what lies at a choice without an expert counts for nothing)
+    out = (torch.where(kept, rows, zero.to(y.dtype)) * torch.where(kept, weights[..., None], zero)).sum(1)
     return (out if residual is None else residual + out).to(y.dtype)
 
 

@@ -1316,3 +1316,22 @@ def test_route_takes_one_expert_with_strides(dtype):
     assert ids[3] == -1 and weights.sum() == 36 and plan.offsets.tolist() == [0, 36]
     weights.backward(torch.randn_like(weights))
     assert not leaf.grad.any()  # the only expert's weight is 1 whatever its logit
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_what_lies_at_choices_without_an_expert_counts_for_nothing(device):
+    """Infinite or NaN weights, and gradients of them, at choices that no expert takes."""
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    plan = fn.moe_plan(torch.tensor([[0, -1], [7, 1]], dtype=torch.int32, device=device), 2)
+    y = torch.ones(4, 8, device=device, dtype=dtype).requires_grad_()
+    w = torch.tensor([[0.5, float("nan")], [float("inf"), 2.0]], device=device).requires_grad_()
+    out = fn.moe_combine(y, w, plan)
+    assert out[:, 0].tolist() == [0.5, 2.0]
+    out.sum().backward()
+    assert w.grad.tolist() == [[8.0, 0.0], [0.0, 8.0]] and y.grad[:, 0].tolist() == [0.5, 2.0, 0.0, 0.0]
+    for normalize in (True, False):
+        logits = torch.tensor([[1.0, NINF, NINF], [NINF] * 3], device=device, requires_grad=True)
+        weights, ids, _ = fn.moe_route(logits, 2, normalize)
+        assert ids.tolist() == [[0, -1], [-1, -1]] and weights.tolist() == [[1.0, 0.0], [0.0, 0.0]]
+        weights.backward(torch.tensor([[1.0, float("nan")], [float("inf"), float("nan")]], device=device))
+        assert not logits.grad.any()
