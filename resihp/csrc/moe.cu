@@ -351,6 +351,7 @@ struct MoveArgs {
   const int* used;       // &offsets[experts]: places from here on hold nothing
   int tokens, k, d;
   int* err;
+  int spans;  // scatter, combine's gradient: leading blocks that zero the rows without a pair
 };
 
 // The place of pair (t, j): -1 if it lies outside the rows (recorded), and whether an
@@ -361,6 +362,57 @@ __device__ __forceinline__ int place_of(const MoveArgs& a, int64_t pair, int use
   if (!ok) record_error(a.err, kErrBounds);
   kept = ok && s < used;
   return ok ? s : -1;
+}
+
+// Rows that no pair names, of the kSpan rows from ``span * kSpan`` on, become zeros: a plan made
+// elsewhere may name a row twice or places out of range, and what lies in memory must not reach
+// a weight gradient through the rows it leaves out. One block looks through all places, marks
+// those of its rows and zeros the others; it depends on no other block, and where a plan is
+// whole it writes nothing. It runs beside the blocks that move the rows, first of the grid.
+constexpr int kSpan = 16384;
+
+template <int VEC>
+__device__ __noinline__ void zero_unnamed(const MoveArgs& a, int span) {
+  using R = Row<VEC>;
+  __shared__ __align__(16) uint8_t named[kSpan];
+  const unsigned pairs = unsigned(a.tokens) * unsigned(a.k);  // (at most kMoeMaxPairs)
+  const unsigned first = unsigned(span) * unsigned(kSpan);
+  const unsigned rows = min(unsigned(kSpan), pairs - first);
+  for (int i = threadIdx.x; i < kSpan / 16; i += 256) reinterpret_cast<uint4*>(named)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  auto mark = [&](int s) {
+    const unsigned at = unsigned(s) - first;  // (negative places are far past ``rows``)
+    if (at < rows) named[at] = 1;
+  };
+  // 16-byte loads between the first and last aligned ones, four under way per thread
+  const unsigned lead = min(pairs, unsigned((4 - ((reinterpret_cast<uintptr_t>(a.slots) >> 2) & 3)) & 3));
+  const unsigned quads = (pairs - lead) >> 2;
+  const int4* body = reinterpret_cast<const int4*>(a.slots + lead);
+  if (threadIdx.x < lead) mark(a.slots[threadIdx.x]);
+  for (unsigned i0 = threadIdx.x; i0 < quads; i0 += 4 * 256) {
+    int4 q[4];
+    #pragma unroll
+    for (int u = 0; u < 4; ++u) q[u] = i0 + u * 256 < quads ? body[i0 + u * 256] : make_int4(-1, -1, -1, -1);
+    #pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      mark(q[u].x);
+      mark(q[u].y);
+      mark(q[u].z);
+      mark(q[u].w);
+    }
+  }
+  for (unsigned i = lead + 4 * quads + threadIdx.x; i < pairs; i += 256) mark(a.slots[i]);
+  __syncthreads();
+  bool missing = false;
+  for (unsigned i = threadIdx.x; i < rows / 4; i += 256) missing |= reinterpret_cast<const uint32_t*>(named)[i] != 0x01010101u;
+  for (unsigned i = rows / 4 * 4 + threadIdx.x; i < rows; i += 256) missing |= named[i] == 0;
+  if (!__syncthreads_or(missing)) return;
+  const int vpr = a.d / VEC;
+  for (unsigned r = threadIdx.x >> 5; r < rows; r += 8) {
+    if (named[r]) continue;
+    typename R::Raw* row = static_cast<typename R::Raw*>(a.out) + (int64_t(first) + r) * vpr;
+    for (int v = threadIdx.x & 31; v < vpr; v += 32) row[v] = R::zero();
+  }
 }
 
 // Choices handled together where few rows keep the SMs waiting: their places, then their rows,
@@ -489,13 +541,20 @@ __global__ void __launch_bounds__(256) moe_gather_warp_kernel(MoveArgs a) {
   }
 }
 
-// Copies of a token's row at its pairs' places; zeros where no expert takes the pair.
+// Copies of a token's row at its pairs' places; zeros where no expert takes the pair. (Registers
+// for eight blocks per SM: with 40, which zero_unnamed would take, 7.9 us instead of 7.4 for 4096
+// tokens of two choices, width 2048.)
 template <int VEC, int U>
-__global__ void __launch_bounds__(256) moe_scatter_kernel(MoveArgs a, int lpr) {
+__global__ void __launch_bounds__(256, 8) moe_scatter_kernel(const __grid_constant__ MoveArgs a, int lpr) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
-  const int t = blockIdx.x * (blockDim.x / lpr) + threadIdx.x / lpr;
+  const int block = int(blockIdx.x) - a.spans;
+  if (block < 0) {
+    if (blockIdx.y == 0) zero_unnamed<VEC>(a, blockIdx.x);
+    return;
+  }
+  const int t = block * (blockDim.x / lpr) + threadIdx.x / lpr;
   const int v = blockIdx.y * lpr * U + threadIdx.x % lpr;
   const int vpr = a.d / VEC;
   if (t >= a.tokens || v >= vpr) return;
@@ -522,12 +581,17 @@ __global__ void __launch_bounds__(256) moe_scatter_kernel(MoveArgs a, int lpr) {
 // token with two choices at a time 20.7. The products are summed lane, warp, pair in a fixed
 // order.
 template <int VEC, int U>
-__global__ void __launch_bounds__(256) moe_combine_bwd_kernel(MoveArgs a, int lpr) {
+__global__ void __launch_bounds__(256) moe_combine_bwd_kernel(const __grid_constant__ MoveArgs a, int lpr) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
   __shared__ float part[8];
-  const int64_t pair = int64_t(blockIdx.x) * (256 / lpr) + threadIdx.x / lpr;
+  const int block = int(blockIdx.x) - a.spans;
+  if (block < 0) {
+    zero_unnamed<VEC>(a, blockIdx.x);
+    return;
+  }
+  const int64_t pair = int64_t(block) * (256 / lpr) + threadIdx.x / lpr;
   const int lane = threadIdx.x % lpr;
   const bool live = pair < int64_t(a.tokens) * a.k;
   const int vpr = a.d / VEC;
@@ -604,9 +668,21 @@ void check_move(const MoveArgs& a) {
 template <int VEC, int U>
 void launch_rows(void (*kernel)(MoveArgs, int), const MoveArgs& a, cudaStream_t st) {
   const int vpr = a.d / VEC, lpr = lanes_for(up(vpr, U));
-  const dim3 grid(up(a.tokens, 256 / lpr), up(vpr, lpr * U));
+  const dim3 grid(up(a.tokens, 256 / lpr) + a.spans, up(vpr, lpr * U));
   RESIHP_CHECK(grid.y <= 65535, "moe rows: width too large");
   RESIHP_CUDA_CHECK(launch_pdl(kernel, grid, 256, 0, st, a, lpr));
+}
+
+// The rows without a pair: blocks of zero_unnamed (``a.spans``), or, where they would take longer
+// than the copies beside them, zeros everywhere first. Dispatch of 8192 tokens of eight choices
+// takes, with those blocks, after zeros and without either: width 64 6.9, 5.6 and 2.8 us; 256
+// 10.2, 12.9 and 6.7; 1024 26.1, 43.9 and 25.9; of 32768 tokens, width 64 25.4, 12.7 and 6.5; 256
+// 51, 45 and 27; 1024 107, 172 and 98; 4096 tokens of two choices, width 2048, 7.4, 14.1 and 7.4.
+// Every block reads all places, so beyond 2^22 of them zeros are the cheaper way again.
+void zero_rest(MoveArgs& a, cudaStream_t st) {
+  const int64_t pairs = int64_t(a.tokens) * a.k;
+  if (pairs <= kSpan || (a.d >= 256 && pairs <= (1 << 22))) a.spans = up(pairs, kSpan);
+  else RESIHP_CUDA_CHECK(cudaMemsetAsync(a.out, 0, size_t(pairs) * a.d * sizeof(__nv_bfloat16), st));
 }
 
 // As many warps as their tables (and the block's two) leave within 48 KB: 16 up to 681 experts,
@@ -723,16 +799,17 @@ void moe_plan(const int* ids, int64_t pairs, int start, int experts, int* counts
 
 void moe_scatter(const void* x, const int* slots, const int* used, void* out, int tokens, int k, int d, int* err,
                  cudaStream_t st) {
-  MoveArgs a{x, nullptr, nullptr, nullptr, out, nullptr, slots, used, tokens, k, d, err};
+  MoveArgs a{x, nullptr, nullptr, nullptr, out, nullptr, slots, used, tokens, k, d, err, 0};
   check_move(a);
   if (tokens == 0) return;
+  zero_rest(a, st);
   if (vectors(a)) launch_rows<8, 1>(moe_scatter_kernel<8, 1>, a, st);
   else launch_rows<1, 4>(moe_scatter_kernel<1, 4>, a, st);
 }
 
 void moe_gather(const void* y, const float* weights, const void* residual, const int* slots, const int* used, void* out,
                 int tokens, int k, int d, int* err, int num_sms, cudaStream_t st) {
-  MoveArgs a{y, nullptr, weights, residual, out, nullptr, slots, used, tokens, k, d, err};
+  MoveArgs a{y, nullptr, weights, residual, out, nullptr, slots, used, tokens, k, d, err, 0};
   check_move(a);
   if (tokens == 0) return;
   const bool many = tokens >= num_sms * 16;
@@ -747,13 +824,14 @@ void moe_gather(const void* y, const float* weights, const void* residual, const
 
 void moe_combine_bwd(const void* dout, const void* y, const float* weights, const int* slots, const int* used, void* dy,
                      float* dweights, int tokens, int k, int d, int* err, int num_sms, cudaStream_t st) {
-  MoveArgs a{dout, y, weights, nullptr, dy, dweights, slots, used, tokens, k, d, err};
+  MoveArgs a{dout, y, weights, nullptr, dy, dweights, slots, used, tokens, k, d, err, 0};
   check_move(a);
   if (tokens == 0) return;
   const bool vec = vectors(a);
   const int vpr = vec ? d / 8 : d;
   const int lpr = int64_t(tokens) * k >= int64_t(num_sms) * 16 ? 32 : std::max(32, lanes_for(vpr));
-  const int grid = up(int64_t(tokens) * k, 256 / lpr);
+  zero_rest(a, st);
+  const int grid = up(int64_t(tokens) * k, 256 / lpr) + a.spans;
   auto kernel = vec ? (vpr <= lpr ? moe_combine_bwd_kernel<8, 1> : moe_combine_bwd_kernel<8, 4>) : moe_combine_bwd_kernel<1, 4>;
   RESIHP_CUDA_CHECK(launch_pdl(kernel, grid, 256, 0, st, a, lpr));
 }

@@ -39,8 +39,9 @@ class MoePlan(NamedTuple):
     ``offsets`` (int32 ``[E + 1]``): expert ``e`` owns the rows ``offsets[e] .. offsets[e + 1]``.
     ``slots`` (int32 ``[T, k]``): each pair's row; pairs of no expert have the rows from
     ``offsets[E]`` on. Every row belongs to exactly one pair; a plan made elsewhere has to keep
-    that (of two pairs with one place either may win). Places outside the rows are left out,
-    and on the kernels reported by :func:`resihp.ops.check_device_errors`.
+    that. Where it does not, rows without a pair are zeros, of two pairs with one place either
+    may win, and places outside the rows are left out and on the kernels reported by
+    :func:`resihp.ops.check_device_errors`.
     """
 
     offsets: torch.Tensor

@@ -1335,3 +1335,50 @@ def test_what_lies_at_choices_without_an_expert_counts_for_nothing(device):
         assert ids.tolist() == [[0, -1], [-1, -1]] and weights.tolist() == [[1.0, 0.0], [0.0, 0.0]]
         weights.backward(torch.tensor([[1.0, float("nan")], [float("inf"), float("nan")]], device=device))
         assert not logits.grad.any()
+
+
+@gpu
+@pytest.mark.parametrize("spoil", ["outside", "twice", "whole"])
+@pytest.mark.parametrize("t,k,d", [(1, 1, 8), (2, 2, 512), (37, 5, 1003), (500, 3, 72), (4001, 5, 128), (9000, 2, 1024),
+                                   (4100, 4, 1027), (2500, 2, 2048)])
+def test_rows_that_no_pair_names_are_zeros(t, k, d, spoil):
+    """A plan made elsewhere that leaves rows out: what lay in memory is in no output."""
+    g = torch.Generator().manual_seed(t + d)
+    n = t * k
+    places = torch.randperm(n, generator=g).to(torch.int32)
+    if spoil != "whole":
+        hit = torch.randperm(n, generator=g)[: max(1, n // 50)]
+        places[hit] = torch.tensor([-1, n, 2**31 - 1, -(2**31)], dtype=torch.int32)[torch.arange(len(hit)) % 4] if spoil == "outside" \
+            else places[torch.randperm(n, generator=g)[: len(hit)]]
+    slots = torch.empty(n + 1, dtype=torch.int32, device="cuda")[1:].view(t, k)  # four bytes behind an aligned address
+    slots.copy_(places.view(t, k))
+    used = n - n // 10
+    plan = fn.MoePlan(torch.tensor([0, n // 2, used], dtype=torch.int32, device="cuda"), slots)
+    at, token = places.long().cuda(), torch.arange(n, device="cuda") // k
+    inside = (at >= 0) & (at < n)
+    times = torch.zeros(n, device="cuda").index_add_(0, at[inside], torch.ones(int(inside.sum()), device="cuda"))
+    once = torch.zeros(n, dtype=torch.bool, device="cuda")
+    once[at[inside]] = True
+    once &= (times == 1) & (torch.arange(n, device="cuda") < used)
+    owner = torch.zeros(n, dtype=torch.int64, device="cuda")
+    owner[at[inside]] = token[inside]
+    check_device_errors()
+
+    def poison():
+        torch.full((n, d), float("nan"), device="cuda", dtype=torch.bfloat16)  # and freed: the next output's memory
+
+    x = torch.randn(t, d, device="cuda").bfloat16()
+    poison()
+    rows = fn.moe_dispatch(x, plan)
+    assert torch.equal(rows[once], x[owner[once]]) and not rows[times == 0].any() and not rows[used:].any()
+    assert rows.isfinite().all()
+    y = torch.randn(n, d, device="cuda").bfloat16().requires_grad_()
+    out = fn.moe_combine(y, torch.ones(t, k, device="cuda"), plan)
+    poison()
+    out.backward(x)
+    assert torch.equal(y.grad[once], x[owner[once]]) and not y.grad[times == 0].any() and not y.grad[used:].any()
+    assert y.grad.isfinite().all()
+    if spoil == "outside":
+        with pytest.raises(KernelError):
+            check_device_errors()
+    check_device_errors()
