@@ -333,10 +333,11 @@ __device__ __forceinline__ void l2_prefetch_bulk(const void* src, uint32_t bytes
 
 // A tile from this CTA's shared memory to its place in a 3-D tensor map (stored, or, fp32, added
 // element by element), in the thread's current bulk group. What lies past the map's edges is left
-// out; ``x`` is a multiple of 16 bytes (4 elements of fp32, 8 of bf16) and nothing is negative.
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z,
+// out; ``x`` is a multiple of 16 bytes (``unit`` elements: 4 of fp32, 8 of bf16) and nothing is
+// negative.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z, int unit,
                                              int* err = nullptr) {
-  if (!bounds_ok((x & 3) == 0 && x >= 0 && y >= 0 && z >= 0 && (smem_u32(src) & 127u) == 0, err)) return;
+  if (!bounds_ok((x & (unit - 1)) == 0 && x >= 0 && y >= 0 && z >= 0 && (smem_u32(src) & 127u) == 0, err)) return;
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
                "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)

@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
           __syncwarp();
           if (lane == 0) {
             if (ACC) tma_add_3d_f32(&tma_c, buf, col0 + j, row0, e, g.err);
-            else tma_store_3d(&tma_c, buf, col0 + j, row0, e, g.err);
+            else tma_store_3d(&tma_c, buf, col0 + j, row0, e, BF16 ? 8 : 4, g.err);
             bulk_commit();
           }
         }

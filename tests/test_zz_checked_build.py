@@ -70,3 +70,49 @@ def test_checked_library_passes_its_checks_and_matches_bitwise():
         results[flag] = json.loads(out.stdout.strip().splitlines()[-1])
     assert results["1"]["lib"].endswith("_C_checked.so") and results["0"]["lib"].endswith("_C.so")
     assert results["1"]["digest"] == results["0"]["digest"]
+
+
+_GROUPED_WORKLOAD = r"""
+import hashlib, itertools, json
+import torch
+from resihp.ops import _ext, check_device_errors, grouped_dgrad, grouped_linear, grouped_wgrad
+from resihp.ops import functional as fn
+torch.manual_seed(0)
+digest = {}
+
+def keep(name, t):
+    digest[name] = hashlib.sha256(t.detach().float().cpu().numpy().tobytes()).hexdigest()
+
+# empty groups, groups cut at every remainder of a step and a tile, rows behind the last group, tiles
+# past the matrices' edges; the last case is one whose CTA pairs keep step
+for sizes, tail, n, k in (([3, 0, 4], 2, 72, 136), ([65, 63, 1, 0, 127, 129, 16, 15], 7, 200, 328), ([5] * 70, 0, 64, 40),
+                          ([700, 1, 900, 257], 129, 1032, 520), ([3000, 1100], 100, 2568, 7176)):
+    offsets = torch.tensor([0, *itertools.accumulate(sizes)], dtype=torch.int32, device="cuda")
+    rows = sum(sizes) + tail
+    x, dy = torch.randn(rows, k, device="cuda").bfloat16(), torch.randn(rows, n, device="cuda").bfloat16()
+    w = torch.randn(len(sizes), n, k, device="cuda").bfloat16()
+    acc = torch.randn(w.shape, device="cuda")
+    name = f"{len(sizes)} {n} {k} "
+    keep(name + "y", grouped_linear(x, w, offsets))
+    keep(name + "dx", grouped_dgrad(dy, w, offsets))
+    keep(name + "dw", grouped_wgrad(dy, x, offsets))
+    keep(name + "accumulated", grouped_wgrad(dy, x, offsets, out=acc, accumulate=True))
+    leaf = w.clone().requires_grad_()
+    fn.grouped_linear(x, leaf, offsets).backward(dy)
+    keep(name + "bf16", leaf.grad)
+torch.cuda.synchronize()
+check_device_errors(0)
+print(json.dumps({"lib": _ext._LIB, "digest": digest}))
+"""
+
+
+@pytest.mark.gpu
+def test_checked_library_passes_its_checks_of_grouped_products():
+    results = {}
+    for flag in ("0", "1"):
+        out = subprocess.run([sys.executable, "-c", _GROUPED_WORKLOAD], capture_output=True, text=True, cwd=ROOT,
+                             env={**os.environ, "RESIHP_CHECKED": flag}, timeout=600)
+        assert out.returncode == 0, out.stderr[-2000:]
+        results[flag] = json.loads(out.stdout.strip().splitlines()[-1])
+    assert results["1"]["lib"].endswith("_C_checked.so") and results["0"]["lib"].endswith("_C.so")
+    assert results["1"]["digest"] == results["0"]["digest"] and len(results["0"]["digest"]) == 25
