@@ -441,17 +441,6 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
-// The same from a 3-D map.
-__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y,
-                                                 int z, int* err = nullptr) {
-  if (!bounds_ok((x & 7) == 0 && x >= 0 && y >= 0 && z >= 0 && (smem_u32(dst) & 1023u) == 0, err)) return;
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-
 // Called by the same warp of both CTAs: ``ncols`` TMEM columns in each, at one address.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
@@ -606,7 +595,7 @@ __device__ __forceinline__ bool wait_geq(const unsigned* p, unsigned target, int
   return true;
 }
 
-// ---- GEMM tiles and epilogues -----------------------------------------------------------
+// ---- GEMM tiles -------------------------------------------------------------------------
 
 // Output tile t of a tiles_m x tiles_n grid, eight tile rows at a time: the tiles that run
 // together share operand tiles in L2.
@@ -619,14 +608,6 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
   const int in_group = t % per_group;
   tm = first + in_group % size;
   tn = in_group / size;
-}
-
-// Fire-and-forget C[0..3] += v in L2. Every element of C is added to by exactly one
-// thread of one CTA per launch, so the sum is the same single fp32 addition the
-// load-add-store epilogue performs (atomic f32 adds flush subnormals to zero).
-__device__ __forceinline__ void red_add_v4(float* p, float4 v) {
-  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-               : "memory");
 }
 
 // ---- AdamW, one element (torch.optim.AdamW's formulation) -----------------------------

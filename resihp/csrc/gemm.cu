@@ -37,6 +37,14 @@ enum GemmEpilogue : int {
   kEpiRedF32 = 4,      // C(f32) += alpha * acc   (red.global.add: no load latency in the epilogue)
 };
 
+// Fire-and-forget C[0..3] += v in L2. Every element of C is added to by exactly one
+// thread of one CTA per launch, so the sum is the same single fp32 addition the
+// load-add-store epilogue performs (atomic f32 adds flush subnormals to zero).
+__device__ __forceinline__ void red_add_v4(float* p, float4 v) {
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+
 struct GemmArgs {
   void* c;
   const void* r;

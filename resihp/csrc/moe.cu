@@ -6,7 +6,8 @@
 //             among equal ones), weights = softmax over all experts or over the chosen ones
 //   plan      offsets[e] = pairs of the experts before e;  slots[t, j] = the pair's place in
 //             the order (expert, token, choice); pairs of no expert go behind offsets[E]
-//   scatter   y[slots[t, j]] = w[t, j] x[t]                (dispatch; combine's gradient)
+//   scatter   y[slots[t, j]] = x[t]                        (dispatch; combine's gradient
+//             y[slots[t, j]] = w[t, j] x[t] goes with its dot products)
 //   gather    out[t] = residual[t] + sum_j w[t, j] y[slots[t, j]]   (combine; dispatch's)
 //
 // The plan is a stable counting sort in two launches: the first counts experts per run of
@@ -343,7 +344,7 @@ struct Row<1> {
 struct MoveArgs {
   const void* in;        // scatter: x / dout [tokens, d]; gather: y [rows, d]
   const void* y;         // scatter: the rows whose product with dout is dweights, or nullptr
-  const float* weights;  // [tokens, k] or nullptr (ones)
+  const float* weights;  // [tokens, k]; gather: or nullptr (ones)
   const void* residual;  // gather: [tokens, d] or nullptr
   void* out;
   float* dweights;
@@ -604,7 +605,7 @@ __global__ void __launch_bounds__(256) moe_combine_bwd_kernel(const __grid_const
     const Raw* y = static_cast<const Raw*>(a.y) + int64_t(s) * vpr;
     Raw* dy = static_cast<Raw*>(a.out) + int64_t(s) * vpr;
     if (kept) {
-      const float w = a.weights != nullptr ? a.weights[pair] : 1.f;
+      const float w = a.weights[pair];
       for (int v0 = lane; v0 < vpr; v0 += U * lpr) {
         Raw gr[U], yr[U];
         #pragma unroll

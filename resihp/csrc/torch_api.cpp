@@ -435,7 +435,7 @@ torch::Tensor moe_gather_t(torch::Tensor y, c10::optional<torch::Tensor> weights
   return out;
 }
 
-std::vector<torch::Tensor> moe_combine_bwd_t(torch::Tensor dout, torch::Tensor y, c10::optional<torch::Tensor> weights,
+std::vector<torch::Tensor> moe_combine_bwd_t(torch::Tensor dout, torch::Tensor y, torch::Tensor weights,
                                              torch::Tensor offsets, torch::Tensor slots) {
   check_plan(dout, offsets, slots);
   check_rows(dout, y.size(-1), "dout");
