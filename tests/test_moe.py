@@ -1382,3 +1382,87 @@ def test_rows_that_no_pair_names_are_zeros(t, k, d, spoil):
         with pytest.raises(KernelError):
             check_device_errors()
     check_device_errors()
+
+
+def _check_moves(t, k, d, with_residual, seed):
+    """Dispatch and combine with their gradients, all rows, against 64-bit sums (on the GPU, by rows)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    ids = make_ids(t, max(k, 6), k, seed).cuda()
+    plan = fn.moe_plan(ids, max(k, 6))
+    at, kept = plan.slots.long(), (ids >= 0)[..., None]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").bfloat16()
+
+    x, dy = normal(t, d).requires_grad_(), normal(t * k, d)
+    rows = fn.moe_dispatch(x, plan)
+    assert torch.equal(rows.detach()[at.reshape(-1)].view(t, k, d), torch.where(kept, x.detach()[:, None], torch.zeros_like(x[:, None])))
+    rows.backward(dy)
+    total, size = torch.zeros(2, t, d, device="cuda", dtype=torch.float64)
+    for j in range(k):
+        part = dy[at[:, j]].double() * kept[:, j]
+        total += part
+        size += part.abs()
+    near(x.grad, total, BF * total.abs() + (k + 1) * F32 * size)
+    y, w, dout = normal(t * k, d).requires_grad_(), torch.rand(t, k, generator=g, device="cuda").requires_grad_(), normal(t, d)
+    r = normal(t, d).requires_grad_() if with_residual else None
+    out = fn.moe_combine(y, w, plan, residual=r)
+    out.backward(dout)
+    want = r.detach().double() if with_residual else torch.zeros(t, d, device="cuda", dtype=torch.float64)
+    size = want.abs()
+    for j in range(k):
+        row, weight = y.detach()[at[:, j]].double() * kept[:, j], w.detach()[:, j, None].double()
+        want, size = want + weight * row, size + (weight * row).abs()
+        dots = row * dout.double()
+        near(w.grad[:, j], dots.sum(1), (d + 8) * F32 * dots.abs().sum(1))
+        back = weight * dout.double() * kept[:, j]
+        near(y.grad[at[:, j]], back, (BF + 2 * F32) * back.abs())
+    near(out, want, BF * want.abs() + 2 * (2 * k + 2) * F32 * size)
+    if with_residual:
+        assert torch.equal(r.grad, dout)
+    check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("t,k,d", [(2400, 2, 256), (2400, 1, 2048), (4096, 2, 1032), (2401, 5, 520), (2400, 3, 64),
+                                   (2500, 2, 1003), (8200, 2, 128)])
+def test_moves_of_many_tokens(t, k, d, with_residual):
+    """A warp per token or pair: row widths of one and several rounds of a warp, even and odd counts
+    of choices."""
+    _check_moves(t, k, d, with_residual, t + d)
+
+
+@gpu
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("t,e,k,dtype", [(5000, 8, 2, torch.bfloat16), (4097, 61, 6, torch.float32), (30000, 64, 4, torch.bfloat16),
+                                         (100_003, 16, 1, torch.float32), (3000, 300, 16, torch.bfloat16), (2000, 1024, 3, torch.float32)])
+def test_route_of_many_tokens(t, e, k, dtype, normalize):
+    """More rows than one block takes, and more blocks than one."""
+    g = torch.Generator().manual_seed(t)
+    logits = (2 * torch.randn(t, e, generator=g)).to(dtype)
+    logits[torch.rand(t, e, generator=g) < 0.3] = NINF
+    logits[::97] = NINF
+    leaf = logits.cuda().requires_grad_()
+    weights, ids, plan = fn.moe_route(leaf, k, normalize)
+    x = logits.double()
+    top, order = x.sort(dim=1, descending=True, stable=True)
+    chosen = torch.where(top[:, :k] == NINF, -1, order[:, :k])
+    assert torch.equal(ids.cpu().long(), chosen)
+    among = torch.zeros(t, e, dtype=torch.bool).scatter_(1, order[:, :k], True) & (x != NINF) if normalize else x != NINF
+    probs = torch.where(among, x, torch.full_like(x, NINF)).softmax(1).nan_to_num(0.0)
+    w64 = probs.gather(1, chosen.clamp_min(0)) * (chosen >= 0)
+    near(weights, w64, (90 + e) * F32 * w64 + 1e-37)
+    key = torch.where(chosen < 0, e, chosen).reshape(-1)
+    slots = torch.empty(t * k, dtype=torch.int64)
+    slots[key.argsort(stable=True)] = torch.arange(t * k)
+    assert torch.equal(plan.slots.cpu().long().reshape(-1), slots)
+    assert plan.offsets.tolist() == [0] + torch.bincount(key, minlength=e + 1)[:e].cumsum(0).tolist()
+    again = fn.moe_plan(ids, e)
+    assert torch.equal(again.slots, plan.slots) and torch.equal(again.offsets, plan.offsets)
+    dw = torch.randn(t, k, generator=g)
+    weights.backward(dw.cuda())
+    up = torch.zeros_like(probs).scatter_add_(1, chosen.clamp_min(0), dw.double() * (chosen >= 0))
+    want = probs * (up - (probs * up).sum(1, keepdim=True))
+    size = probs * (up.abs() + (probs * up.abs()).sum(1, keepdim=True))
+    near(leaf.grad, want, (BF * want.abs() if dtype == torch.bfloat16 else 0) + (300 + 4 * e) * F32 * size + 1e-37)
