@@ -51,8 +51,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = Non
     lead = x.shape[:-1]
     x2 = x.reshape(-1, x.shape[-1])
     out = torch.empty((x2.shape[0], w.shape[0]), dtype=torch.bfloat16, device=x.device)
-    if not out.shape[0]:  # no rows: nothing to launch
-        pass
+    if not out.shape[0] and x2.shape[1] == w.shape[1]:
+        pass  # no rows: nothing to launch
     elif residual is None:
         _ext.require().gemm(x2, False, w, False, out, EPI_BF16)
     else:
@@ -68,7 +68,7 @@ def linear_dgrad(dy: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     lead = dy.shape[:-1]
     d2 = dy.reshape(-1, dy.shape[-1])
     out = torch.empty((d2.shape[0], w.shape[1]), dtype=torch.bfloat16, device=dy.device)
-    if out.shape[0]:
+    if out.shape[0] or d2.shape[1] != w.shape[0]:
         _ext.require().gemm(d2, False, w, True, out, EPI_BF16)
     return out.view(*lead, w.shape[1])
 
@@ -94,7 +94,7 @@ def linear_wgrad(dy: torch.Tensor, x: torch.Tensor, out: torch.Tensor | None = N
     if out is None:
         out = torch.empty((d2.shape[1], x2.shape[1]), dtype=torch.float32, device=dy.device)
         accumulate = False
-    if not d2.shape[0]:  # no rows: a sum of nothing
+    if d2.shape[0] == x2.shape[0] == 0 and out.shape == (d2.shape[1], x2.shape[1]):  # a sum of nothing
         return out if accumulate else out.zero_()
     _ext.require().gemm(d2, True, x2, True, out, ((EPI_RED_F32 if WGRAD_RED else EPI_ACC_F32) if accumulate
                                                  else EPI_F32))

@@ -1466,3 +1466,76 @@ def test_route_of_many_tokens(t, e, k, dtype, normalize):
     want = probs * (up - (probs * up).sum(1, keepdim=True))
     size = probs * (up.abs() + (probs * up.abs()).sum(1, keepdim=True))
     near(leaf.grad, want, (BF * want.abs() if dtype == torch.bfloat16 else 0) + (300 + 4 * e) * F32 * size + 1e-37)
+
+
+@gpu
+def test_linear_products_without_rows_are_checked():
+    x, w = torch.empty(0, 16, device="cuda").bfloat16(), torch.randn(24, 8, device="cuda").bfloat16()
+    rows = torch.randn(8, 16, device="cuda").bfloat16()
+    for call in (lambda: fn.linear(x, w), lambda: fn.linear_dgrad(x, w), lambda: fn.linear_wgrad(x, rows),
+                 lambda: fn.linear_wgrad(x, x[:, :8], out=torch.zeros(16, 16, device="cuda"))):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@gpu
+def test_captured_block_without_accumulators():
+    """Every weight's own gradient in a graph, replayed on other rows."""
+    leaves = [t.requires_grad_() for t in _block(15)]
+
+    def step():
+        out = fn.moe_swiglu(*leaves, 2, residual=leaves[0])
+        return (out.detach(), *torch.autograd.grad(out, leaves, out.detach()))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (16, 17):
+        with torch.no_grad():
+            leaves[0].copy_(_block(seed)[0])
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+    check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("d", [128, 256])
+def test_captured_moves_of_plans_that_change(d):
+    """The places are read at each replay, whole or with rows left out (both ways to zero those)."""
+    t, k = 9000, 2
+    x, y = torch.randn(t, d, device="cuda").bfloat16(), torch.randn(t * k, d, device="cuda").bfloat16().requires_grad_()
+    slots = torch.arange(t * k, dtype=torch.int32, device="cuda").view(t, k).clone()
+    plan = fn.MoePlan(torch.tensor([0, t * k], dtype=torch.int32, device="cuda"), slots)
+    weights = torch.rand(t, k, device="cuda")
+
+    def step():
+        out = fn.moe_combine(y, weights, plan)
+        return fn.moe_dispatch(x, plan), torch.autograd.grad(out, y, x)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rows, dy = step()
+    for left_out in (0, 700, 0):
+        slots.copy_(torch.randperm(t * k, device="cuda").view(t, k))
+        if left_out:
+            gone = slots.view(-1)[:left_out].long()
+            slots.view(-1)[:left_out] = slots.view(-1)[left_out: 2 * left_out]  # named twice, so others not at all
+        rows.fill_(float("nan")), dy.fill_(float("nan"))
+        graph.replay()
+        assert rows.isfinite().all() and dy.isfinite().all()
+        last = slots.view(-1)[2 * left_out:].long()
+        token = torch.arange(2 * left_out, t * k, device="cuda") // k
+        assert torch.equal(rows[last], x[token])
+        if left_out:
+            assert not rows[gone].any() and not dy[gone].any()
+    check_device_errors()
