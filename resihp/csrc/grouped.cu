@@ -159,8 +159,10 @@ __device__ __forceinline__ RowSpan span_of(const Lists& l, int e, int t, int til
 // same bytes again from memory: 16384 rows, 13824 > 5120, eight uneven groups, brought 7.7 GB
 // in where 1.6 are needed, and the last pair ended 18 % after the first. Where the panels of a
 // round pass half of L2 (k from 7168 on) every pair therefore counts itself in each 64 K
-// blocks, and waits a moment while another is two such steps behind: 1122 -> 1220 TF/s
-// there under the power cap; at k = 5504 and 11008 (8192 rows) it neither gains nor costs.
+// blocks, and waits a moment while the pairs' steps add up to fewer than its own times the number
+// of pairs. That bounds how far a pair runs ahead of the average, not of the slowest: one straggler
+// holds nobody up. 1122 -> 1220 TF/s there under the power cap; at k = 5504 and 11008
+// (8192 rows), the only other depths it was timed at, it neither gains nor costs.
 constexpr int kPaceBlocks = 64;
 constexpr int kPaceDepth = 7168;
 constexpr uint64_t kPaceNs = 20000;
