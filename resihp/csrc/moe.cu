@@ -369,11 +369,13 @@ __device__ __forceinline__ int place_of(const MoveArgs& a, int64_t pair, int use
 // elsewhere may name a row twice or places out of range, and what lies in memory must not reach
 // a weight gradient through the rows it leaves out. One block looks through all places, marks
 // those of its rows and zeros the others; it depends on no other block, and where a plan is
-// whole it writes nothing. It runs beside the blocks that move the rows, first of the grid.
+// whole it writes nothing. It runs beside the blocks that move the rows, first of the grid. (Inline:
+// behind a call the movers lose a tenth at odd widths. Marks are bytes: bits need atomics, twice
+// the time.)
 constexpr int kSpan = 16384;
 
 template <int VEC>
-__device__ __noinline__ void zero_unnamed(const MoveArgs& a, int span) {
+__device__ __forceinline__ void zero_unnamed(const MoveArgs& a, int span) {
   using R = Row<VEC>;
   __shared__ __align__(16) uint8_t named[kSpan];
   const unsigned pairs = unsigned(a.tokens) * unsigned(a.k);  // (at most kMoeMaxPairs)
@@ -543,10 +545,10 @@ __global__ void __launch_bounds__(256) moe_gather_warp_kernel(MoveArgs a) {
 }
 
 // Copies of a token's row at its pairs' places; zeros where no expert takes the pair. (Registers
-// for eight blocks per SM: with 40, which zero_unnamed would take, 7.9 us instead of 7.4 for 4096
+// for eight blocks per SM: with the 40 that zero_unnamed would take, 7.9 us instead of 7.4 for 4096
 // tokens of two choices, width 2048.)
 template <int VEC, int U>
-__global__ void __launch_bounds__(256, 8) moe_scatter_kernel(const __grid_constant__ MoveArgs a, int lpr) {
+__global__ void __launch_bounds__(256, 8) moe_scatter_kernel(MoveArgs a, int lpr) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
@@ -582,7 +584,7 @@ __global__ void __launch_bounds__(256, 8) moe_scatter_kernel(const __grid_consta
 // token with two choices at a time 20.7. The products are summed lane, warp, pair in a fixed
 // order.
 template <int VEC, int U>
-__global__ void __launch_bounds__(256) moe_combine_bwd_kernel(const __grid_constant__ MoveArgs a, int lpr) {
+__global__ void __launch_bounds__(256) moe_combine_bwd_kernel(MoveArgs a, int lpr) {
   pdl_enter();
   using R = Row<VEC>;
   using Raw = typename R::Raw;
@@ -677,7 +679,7 @@ void launch_rows(void (*kernel)(MoveArgs, int), const MoveArgs& a, cudaStream_t 
 // The rows without a pair: blocks of zero_unnamed (``a.spans``), or, where they would take longer
 // than the copies beside them, zeros everywhere first. Dispatch of 8192 tokens of eight choices
 // takes, with those blocks, after zeros and without either: width 64 6.9, 5.6 and 2.8 us; 256
-// 10.2, 12.9 and 6.7; 1024 26.1, 43.9 and 25.9; of 32768 tokens, width 64 25.4, 12.7 and 6.5; 256
+// 10.8, 12.9 and 6.8; 1024 26.1, 43.9 and 25.9; of 32768 tokens, width 64 25.4, 12.7 and 6.5; 256
 // 51, 45 and 27; 1024 107, 172 and 98; 4096 tokens of two choices, width 2048, 7.4, 14.1 and 7.4.
 // Every block reads all places, so beyond 2^22 of them zeros are the cheaper way again.
 void zero_rest(MoveArgs& a, cudaStream_t st) {
