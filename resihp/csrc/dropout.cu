@@ -92,10 +92,11 @@ __device__ __forceinline__ T drop_one(T x, T res, const uint32_t (&w)[4], int e,
 
 // Whole blocks as 16-byte vectors (element 0 starts a block, aligned pointers). A thread takes
 // two blocks of a 512-block tile, at fixed distances: one address computation, both loads under
-// way during the integer work. What bounds it is that work, not the memory: twenty 32 x 32 > 64
-// bit products per block. Ten rounds take 60 us, five would take 55 and none 53 (16384 x 5120
-// bf16, 335 MB moved, 5.6 TB/s of the 6.5 a copy reaches). The round keys come from the kernel's constants, so a round is
-// two products and two three-way exclusive ors. DROP false (p below 2^-17): nothing is drawn.
+// way during the integer work (twenty 32 x 32 > 64 bit products per block), which adds 14 % to
+// the memory's time: ten rounds take 60 us, five would take 55 and none 53 (16384 x 5120 bf16, 335
+// MB moved, 5.6 TB/s of the 6.5 a copy reaches). The round keys come from the kernel's constants,
+// so a round is two products and two three-way exclusive ors. DROP false (p below 2^-17): nothing
+// is drawn.
 constexpr int kTile = 512;
 
 template <typename T, bool DROP, bool RES, bool STATE>

@@ -118,9 +118,13 @@ __device__ __forceinline__ int group_of(const Lists& l, int groups, int t, int f
 // more than TN rows is cut into equal parts, not into full tiles and a rest.
 //
 // Many rows: bound by the tensor cores, and in long products by the power cap: 8192 rows of
-// eight groups, 2048 > 11008, take 270 us forward and 266 backward (1366 and 1390 TF/s of the
+// eight groups, 2048 > 11008, take 268 us forward and 280 backward (1376 and 1319 TF/s of the
 // 1643 a library product reaches in a burst, 1397 sustained). Few rows: bound by reading the
-// weights: 16 rows, same weights, 58 us (6.2 TB/s of the 6.5 a copy reaches).
+// weights: 16 rows, same weights, 60 us (6.0 TB/s of the 6.5 a copy reaches).
+//
+// One accumulator takes the whole depth, with the truncating additions that the weight gradient
+// below cuts short: at most 2e-5 of the norm at these depths, where the output's rounding to bf16 is
+// 1.7e-3. It moves 0.1 % of the outputs (k 2048) to 0.8 % (k 13824) across a rounding's border.
 
 constexpr int kBK = 64;
 
@@ -374,9 +378,10 @@ __global__ void __launch_bounds__(192, 1)
 // warps per CTA keep 128 columns of a row per thread. The finished tile leaves through shared
 // memory as bulk stores or bulk additions (whole 128-byte runs, clipped at the matrix's edges
 // by the map): each element is added to once per launch, so no order can change the sum.
-// 8192 rows of eight groups, 2048 x 11008: 345 us written, 388 added to what is there (721 MB
+// 8192 rows of eight groups, 2048 x 11008: 322 us written, 374 added to what is there (721 MB
 // of fp32, of which the sums alone would take 110 us and 220; the MMAs 270). As a bf16 gradient,
-// rounded once from the fp32 sum, 265 us; written in fp32 and cast by another kernel 440.
+// rounded once from the fp32 sum, 283 us; written in fp32 and cast by another kernel 440. With the
+// GPU at its power cap, after other long products, 360, 410 to 430 and 265 to 300.
 //
 // A group's last block holds rows of the next group where its length is no multiple of 64.
 // Steps of 16 rows past the end are not issued; rows past the end inside the last step are
@@ -473,7 +478,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
   if (warp == 0 || warp == 11) {
     // Two producers, one per operand: a load costs its warp about 120 cycles, and four of them
     // per block would pace the MMAs (512 cycles; 8192 rows, 2048 x 11008, eight groups, written:
-    // 370 us with one producer, 345 with two). The whole warp walks, one lane issues.
+    // 370 us with one producer, 345 with two, then). The whole warp walks, one lane issues.
     const bool second = warp == 11;
     const uint32_t issue = elect_one(), lead = cta == 0 && !second ? issue : 0u, own = second ? 0u : issue;
     const CUtensorMap* map = second ? &tma_x : &tma_dy;
@@ -776,6 +781,7 @@ void grouped_rows(const void* a, int64_t lda, const void* w, int64_t ldw, int64_
   // eight of their stages in flight instead of six. At 100 rows a group (eight groups, 2048 >
   // 11008) 64.3 against 66.7 us, at 94 uneven ones (64 groups, 1024 > 1416) 44.3 against 46.9;
   // at 150 uneven ones 73.7 against 70.6: groups of more than 128 rows read their weights twice.
+  // The average is all the host knows: how uneven the groups are stands on the device.
   if (s.rows <= int64_t(112) * s.groups) launch_rows_tn<128>(a, lda, w, ldw, w_group, w_mn, s, g, st);
   else launch_rows_tn<256>(a, lda, w, ldw, w_group, w_mn, s, g, st);
 }

@@ -16,11 +16,14 @@
 // (they only count), so a plan is the same on every run; and no state outlives a call.
 //
 // The row movements go by token (or by pair, one token's pairs side by side), so a token's row
-// comes from memory once however many experts it has: k + 1 rows move per token, which is all
-// that has to move. They are bound by memory: at 4096 tokens of two choices, width 2048, dispatch
-// takes 7.0 us, combine 11.4, their gradients 8.4 and 13.5, at 5.9 TB/s and more of the 6.5 a
-// copy reaches. Rows of an odd width have no common alignment and move two bytes at a time: 1021
-// tokens of six choices, width 1003, take 5.6 us out and 9.0 back, where their bytes take 2.2.
+// comes from memory once however many experts it has. Per token k + 1 rows move in dispatch, its
+// gradient and combine (k + 2 with a residual), 2 k + 1 in combine's gradient: no more than has
+// to. They are bound by memory: 4096 tokens of two choices, width 2048, on rows that are not in
+// L2, take 9.4 us for dispatch, 12.8 for combine with a residual, 9.9 and 15.3 for their gradients
+// (5.1 to 5.5 TB/s of the 6.5 a copy reaches); with three sets of rows in turn, partly from L2,
+// 7.2, 11.6, 8.6 and 13.5. Rows of an odd width have no common alignment and move two bytes at a
+// time: 1021 tokens of six choices, width 1003, take 5.7 us out and 10.5 back, where their bytes
+// take 2.2.
 #include <algorithm>
 
 #include "common.cuh"
@@ -481,8 +484,8 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(MoveArgs a, int lpr) {
 // The same with a warp per token, U vectors per lane and J choices under way at a time; the
 // warp's lanes fetch the token's places and weights together and hand them round. Many rows of
 // at least 32 vectors: no block-wide step and no idle lane between a token's loads. 4096 tokens
-// of two choices, width 2048, with residual: 11.4 us (5.9 TB/s) with U = J = 2; U = 4 12.5,
-// J = 4 16.5 (fewer warps), a thread per vector 13.1.
+// of two choices, width 2048, with residual (three sets in turn): 11.4 us with U = J = 2; U = 4
+// 12.5, J = 4 16.5 (fewer warps), a thread per vector 13.1.
 template <int VEC, int U, int J>
 __global__ void __launch_bounds__(256) moe_gather_warp_kernel(MoveArgs a) {
   pdl_enter();
@@ -580,8 +583,8 @@ __global__ void __launch_bounds__(256, 8) moe_scatter_kernel(MoveArgs a, int lpr
 // ``lpr`` lanes per pair (t, j), U vectors per lane at a time: one warp where there are pairs
 // enough to fill the SMs with warps, up to a block where there are few. A token's dout is read
 // once per choice, from the caches after the first. 4096 tokens of two choices, width 2048: a
-// warp per pair 13.7 us (6.1 TB/s; U = 2 14.6, U = 8 16.3), a block per pair 23.6, a block per
-// token with two choices at a time 20.7. The products are summed lane, warp, pair in a fixed
+// warp per pair 13.7 us (three sets in turn; U = 2 14.6, U = 8 16.3), a block per pair 23.6, a
+// block per token with two choices at a time 20.7. The products are summed lane, warp, pair in a fixed
 // order.
 template <int VEC, int U>
 __global__ void __launch_bounds__(256) moe_combine_bwd_kernel(MoveArgs a, int lpr) {
