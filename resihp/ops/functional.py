@@ -237,8 +237,8 @@ def moe_swiglu(x, w_router, w_gate_up, w_down, k, *, normalize=True, residual=No
     dtype), ``w_gate_up [E, 2F, d]`` and ``w_down [E, d, F]`` are the experts' fused gate / up
     and down projections. ``grads``: the FP32 main-grad buffers of the three weights in that
     order (CUDA bf16; see :func:`linear`); a weight without one gets its gradient from
-    autograd. On the kernels the router takes a multiple of 8 experts (its logits are a GEMM's
-    output). The steps are :mod:`resihp.ops.moe`'s.
+    autograd. On the kernels the experts (the router's logits are a GEMM's output), ``d`` and
+    ``F`` are multiples of 8. The steps are :mod:`resihp.ops.moe`'s.
     """
     check_block(x, w_router, w_gate_up, w_down, k, residual, grads)
     g_router, g_gate_up, g_down = grads if grads is not None else (None, None, None)

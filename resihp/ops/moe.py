@@ -15,7 +15,8 @@ behind the last expert's rows, which are zero, and :func:`moe_combine` leaves it
 
 As elsewhere in this package bf16 CUDA tensors run the kernels (``csrc/moe.cu``,
 ``csrc/grouped.cu``) and FP32 rows the plain torch expressions; the router's logits run its
-kernel on every CUDA device in bf16 or FP32. (No counterpart in the reference, whose blocks
+kernel on every CUDA device in bf16 or FP32. FP32 grouped products read ``offsets`` on the
+host, so a step of theirs cannot be captured. (No counterpart in the reference, whose blocks
 are dense.)
 """
 
